@@ -63,6 +63,18 @@ std::vector<at::Tensor> flash_attn_bwd(const at::Tensor& dout, const at::Tensor&
 at::Tensor doc_bounds(const at::Tensor& doc);
 at::Tensor decode_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool causal,
                             int64_t window, double scale);
+std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fresh, at::Tensor& tables,
+                                   const at::Tensor& free_pages, const at::Tensor& free_head, int64_t page_size,
+                                   int64_t n_tokens);
+std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, int64_t n_kv, int64_t D,
+                                           const at::Tensor& qs, const at::Tensor& ks,
+                                           const c10::optional<at::Tensor>& cos_t,
+                                           const c10::optional<at::Tensor>& sin_t, const at::Tensor& positions,
+                                           const at::Tensor& slots, at::Tensor& kp, at::Tensor& vp, double eps,
+                                           bool dense);
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& tables,
+                           const at::Tensor& positions, const c10::optional<at::Tensor>& rows, int64_t window,
+                           const c10::optional<at::Tensor>& slopes, double scale);
 at::Tensor flash_attn_fwd_trace();
 at::Tensor flash_attn_bwd_trace();
 void zero_reduce_scatter(const std::vector<int64_t>& bucket_ptrs, at::Tensor& shard, double scale,
@@ -192,5 +204,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "MINT_FA_TRACE=1 diagnostics: clock64 stamps of the last backward's key tile 0");
   m.def("decode_attention", &mint::decode_attention,
         "split-KV attention of a few query rows against a KV cache prefix (bottom-right causal, window)");
+  m.def("paged_plan", &mint::paged_plan,
+        "block tables, slots and positions of one step from request lengths -> (positions, slots, rows, ends, "
+        "seq_lens, free_head)");
+  m.def("qk_norm_rope_paged", &mint::qk_norm_rope_paged,
+        "QK-norm + rotation at per-token positions, k and v stored into the pages -> (q[, k, v])");
+  m.def("paged_attention", &mint::paged_attention, "attention of single query tokens over a paged KV cache");
   m.def("doc_bounds", &mint::doc_bounds, "[B, T, 2] int32 document run [start, end) of every token");
 }

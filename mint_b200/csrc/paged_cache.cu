@@ -1,0 +1,409 @@
+// Paged key-value cache: the step plan (block tables, slots and positions from request lengths) and
+// the fused QK-norm + rotation + append.
+//
+// A cache layer is two pools [pages, Hkv, page_size, D] (any strides with contiguous D). Slot s is
+// line s % page_size of page s / page_size. Page sizes are powers of two. The reference has a dense
+// [B, Tmax, Hkv, D] cache only (mint/kvcache/base.py:4-65).
+#include <algorithm>
+#include <climits>
+
+#include "paged.cuh"
+
+namespace mint {
+namespace paged {
+
+constexpr int kPlanThreads = 256;
+constexpr int kMaxRequests = 16384;
+// Lengths and prefix sums saturate here, far above any cache, so that a corrupt length cannot wrap an
+// index: 2 * (2^30 - 1) still fits an int.
+constexpr int kLenCap = (1 << 30) - 1;
+
+__device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, kLenCap); }
+__device__ __forceinline__ int clamp_len(int n) { return min(max(n, 0), kLenCap); }
+__device__ __forceinline__ int pages_of(int tokens, int page_shift) {
+  return static_cast<int>((static_cast<unsigned>(tokens) + (1u << page_shift) - 1u) >> page_shift);
+}
+
+// largest r in [0, n) with prefix[r] <= i, for a non-decreasing prefix with prefix[0] = 0 <= i
+__device__ __forceinline__ int last_not_above(const int* prefix, int n, int i) {
+  int lo = 0, hi = n;  // prefix[lo] <= i < prefix[hi] (hi = n stands for the end)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= i) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
+}
+
+struct PlanParams {
+  const int* seq;    // [B] tokens already cached
+  const int* fresh;  // [B] tokens this step
+  int* tables;       // [B, W], row stride tstride
+  const int* free_pages;
+  const int* free_head;
+  int* positions;  // [N]
+  int* slots;      // [N]
+  int* rows;       // [N]
+  int* ends;       // [B]
+  int* seq_out;    // [B]
+  int* head_out;   // [1]
+  uint32_t* status;
+  long long tstride;
+  int B, W, N, n_free, page_shift;
+};
+
+// Every block repeats the prefix sums over the requests (B ints, from L2) and then fills its share of
+// the tokens, tables and request rows, so no block waits for another: a token that falls into a page
+// handed out in this step reads the page id from the free list, not from the table entry that another
+// block writes.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p) {
+  extern __shared__ int s_prefix[];  // [B + 1] tokens before request b, [B + 1] fresh pages before it
+  int* s_tok = s_prefix;
+  int* s_page = s_prefix + p.B + 1;
+  __shared__ int s_warp[2][kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int page_size = 1 << p.page_shift;
+  const int per = (p.B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  bool bad = false;
+  int tok = 0, pages = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int seq = clamp_len(p.seq[b]), add = clamp_len(p.fresh[b]);
+    bad |= p.seq[b] != seq || p.fresh[b] != add;
+    s_tok[b] = add;
+    s_page[b] = pages_of(seq + add, p.page_shift) - pages_of(seq, p.page_shift);
+    tok = sat_add(tok, add);
+    pages = sat_add(pages, s_page[b]);
+  }
+  // exclusive prefix of the threads' sums: within the warp, then over the warps (saturating adds of
+  // non-negative numbers associate)
+  int tok_inc = tok, page_inc = pages;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, tok_inc, d), c = __shfl_up_sync(0xffffffffu, page_inc, d);
+    if (lane >= d) {
+      tok_inc = sat_add(tok_inc, a);
+      page_inc = sat_add(page_inc, c);
+    }
+  }
+  if (lane == 31) {
+    s_warp[0][warp] = tok_inc;
+    s_warp[1][warp] = page_inc;
+  }
+  __syncthreads();
+  int tok_at = __shfl_up_sync(0xffffffffu, tok_inc, 1), page_at = __shfl_up_sync(0xffffffffu, page_inc, 1);
+  if (lane == 0) tok_at = page_at = 0;
+  int tok_sum = 0, page_sum = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) {
+      tok_at = sat_add(tok_at, s_warp[0][w]);
+      page_at = sat_add(page_at, s_warp[1][w]);
+    }
+    tok_sum = sat_add(tok_sum, s_warp[0][w]);
+    page_sum = sat_add(page_sum, s_warp[1][w]);
+  }
+  for (int b = b0; b < b1; ++b) {
+    const int add = s_tok[b], need = s_page[b];
+    s_tok[b] = tok_at;
+    s_page[b] = page_at;
+    tok_at = sat_add(tok_at, add);
+    page_at = sat_add(page_at, need);
+  }
+  if (tid == 0) {
+    s_tok[p.B] = tok_sum;
+    s_page[p.B] = page_sum;
+  }
+  __syncthreads();
+  const int head = *p.free_head;
+  const int left = head < 0 ? 0 : max(0, p.n_free - head);  // pages that can be handed out
+  const int page_cap = INT_MAX >> p.page_shift;              // pages whose slots fit an int
+  bad |= tok_sum > p.N || page_sum > left || head < 0;
+  const int gtid = blockIdx.x * kPlanThreads + tid, gsize = gridDim.x * kPlanThreads;
+
+  for (int i = gtid; i < p.N; i += gsize) {
+    int pos = -1, slot = -1, row = -1;
+    if (i < tok_sum) {
+      row = last_not_above(s_tok, p.B, i);
+      const int seq = clamp_len(p.seq[row]);
+      pos = seq + i - s_tok[row];
+      const int page_no = pos >> p.page_shift;
+      const int have = pages_of(seq, p.page_shift);
+      int page = -1;
+      if (page_no < p.W) {
+        if (page_no < have) {
+          page = p.tables[row * p.tstride + page_no];
+        } else {
+          const int k = s_page[row] + page_no - have;
+          if (k < left) page = p.free_pages[head + k];
+        }
+      }
+      if (page >= 0 && page <= page_cap) {
+        slot = (page << p.page_shift) | (pos & (page_size - 1));
+      } else {
+        bad = true;
+      }
+    }
+    p.positions[i] = pos;
+    p.slots[i] = slot;
+    p.rows[i] = row;
+  }
+  for (int k = gtid; k < page_sum; k += gsize) {
+    const int row = last_not_above(s_page, p.B, k);
+    const int col = pages_of(clamp_len(p.seq[row]), p.page_shift) + k - s_page[row];
+    if (col < p.W) p.tables[row * p.tstride + col] = k < left ? p.free_pages[head + k] : -1;
+  }
+  for (int b = gtid; b < p.B; b += gsize) {
+    p.ends[b] = s_tok[b + 1];
+    p.seq_out[b] = clamp_len(p.seq[b]) + clamp_len(p.fresh[b]);
+  }
+  if (gtid == 0) *p.head_out = head + min(page_sum, left);
+  if (bad) record_status(p.status, kStatusBadArgument);
+}
+
+struct AppendParams {
+  const void* qkv;  // [N, (Hq + 2 Hkv) * D], row stride qkv_stride
+  const float* qs;
+  const float* ks;
+  const float* cos_t;  // [S, D / 2] or null (no rotation)
+  const float* sin_t;
+  const int* positions;
+  const int* slots;
+  void* q;   // [N, Hq, D]
+  void* k;   // [N, Hkv, D] or null
+  void* v;   // [N, Hkv, D] or null
+  void* kp;  // pools
+  void* vp;
+  uint32_t* status;
+  long long qkv_stride, kp_page, kp_head, kp_line, vp_page, vp_head, vp_line;
+  int N, Hq, Hkv, table_len, page_shift, n_pages;
+  float eps;
+};
+
+// D / 8 lanes own one head row: lane l holds elements 8l .. 8l+7 (16-byte accesses), its rotation
+// partner (j +- D / 2) is lane l ^ (D / 16). Norm and rotation in fp32, rounded once on the store.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
+  constexpr int L = D / 8;
+  const int hl = threadIdx.x % L;
+  const int H = p.Hq + 2 * p.Hkv;
+  const long long item = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const bool live = item < static_cast<long long>(p.N) * H;
+  const int m = live ? static_cast<int>(item / H) : 0;
+  const int hh = live ? static_cast<int>(item - static_cast<long long>(m) * H) : 0;
+  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.qkv) + m * p.qkv_stride + hh * D + hl * 8);
+  const int pos = p.positions[m], slot = p.slots[m];
+  const bool is_q = hh < p.Hq, is_v = hh >= p.Hq + p.Hkv;
+  const bool known = pos >= 0 && (p.cos_t == nullptr || pos < p.table_len);
+  const bool stored = known && slot >= 0 && (slot >> p.page_shift) < p.n_pages;
+  if (live && hl == 0 && ((pos >= 0 && !known) || (slot >= 0 && (slot >> p.page_shift) >= p.n_pages)))
+    record_status(p.status, kStatusBadArgument);
+  uint4 out = raw;
+  if (!is_v) {
+    float x[8], w[8];
+    unpack8<T>(raw, x);
+    load8((is_q ? p.qs : p.ks) + hl * 8, w);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    // the butterfly stays inside the row's L lanes; rows of one warp may differ in kind (q, k, v),
+    // so only the row's own lanes take part
+    const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(mask, ss, d);
+    const float r = rsqrtf(ss / D + p.eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= r * (1.f + w[e]);
+    if (p.cos_t != nullptr) {
+      const long long at = static_cast<long long>(known ? pos : 0) * (D / 2) + (hl % (L / 2)) * 8;
+      float c[8], s[8];
+      load8(p.cos_t + at, c);
+      load8(p.sin_t + at, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float partner = __shfl_xor_sync(mask, x[e], L / 2);
+        x[e] = hl < L / 2 ? x[e] * c[e] - partner * s[e] : partner * s[e] + x[e] * c[e];
+      }
+    }
+    out = pack8<T>(x);
+  }
+  if (!known) out = make_uint4(0, 0, 0, 0);
+  if (!live) return;
+  if (is_q) {
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.q) + (static_cast<long long>(m) * p.Hq + hh) * D + hl * 8) = out;
+    return;
+  }
+  const int hk = is_v ? hh - p.Hq - p.Hkv : hh - p.Hq;
+  T* dense = static_cast<T*>(is_v ? p.v : p.k);
+  if (dense != nullptr)
+    *reinterpret_cast<uint4*>(dense + (static_cast<long long>(m) * p.Hkv + hk) * D + hl * 8) = out;
+  if (!stored) return;
+  const long long page = slot >> p.page_shift, line = slot & ((1 << p.page_shift) - 1);
+  T* dst = is_v ? static_cast<T*>(p.vp) + page * p.vp_page + hk * p.vp_head + line * p.vp_line
+                : static_cast<T*>(p.kp) + page * p.kp_page + hk * p.kp_head + line * p.kp_line;
+  *reinterpret_cast<uint4*>(dst + hl * 8) = out;
+}
+
+template <typename T>
+void launch_append(const AppendParams& p, int D, cudaStream_t st) {
+  const long long threads = static_cast<long long>(p.N) * (p.Hq + 2 * p.Hkv) * (D / 8);
+  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+  if (D == 64) {
+    append_kernel<T, 64><<<grid, 256, 0, st>>>(p);
+  } else if (D == 128) {
+    append_kernel<T, 128><<<grid, 256, 0, st>>>(p);
+  } else {
+    append_kernel<T, 256><<<grid, 256, 0, st>>>(p);
+  }
+}
+
+}  // namespace paged
+
+// Plan of one step over B requests: hands out pages from free_pages[free_head ...] to requests whose
+// seq + fresh tokens need more than they have (written into `tables`), and returns positions, slots and
+// request rows of the n_tokens packed tokens (-1 beyond the last), the requests' token ends, their new
+// lengths and the new head of the free list.
+std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fresh, at::Tensor& tables,
+                                   const at::Tensor& free_pages, const at::Tensor& free_head, int64_t page_size,
+                                   int64_t n_tokens) {
+  check_contig(seq, "seq_lens");
+  check_contig(fresh, "new_lens");
+  check_cuda(tables, "block_tables");
+  check_contig(free_pages, "free_pages");
+  check_contig(free_head, "free_head");
+  for (const at::Tensor* t : {&seq, &fresh, static_cast<const at::Tensor*>(&tables), &free_pages, &free_head})
+    MINT_CHECK(t->scalar_type() == at::kInt && t->device() == seq.device(), "paged_plan takes int32 tensors on one device");
+  const int64_t B = seq.numel();
+  MINT_CHECK(fresh.numel() == B && tables.dim() == 2 && tables.size(0) == B && tables.stride(1) == 1,
+             "paged_plan: one length pair and one table row per request");
+  MINT_CHECK(B <= paged::kMaxRequests, "paged_plan takes at most ", paged::kMaxRequests, " requests");
+  MINT_CHECK(free_head.numel() == 1, "free_head has one element");
+  MINT_CHECK(n_tokens >= 0 && n_tokens <= paged::kLenCap && tables.size(1) < (1ll << 31) && free_pages.numel() < (1ll << 31),
+             "paged_plan sizes");
+  auto opts = seq.options();
+  auto tok = at::empty({3, n_tokens}, opts);
+  auto req = at::empty({2, B}, opts);
+  auto head = at::empty({1}, opts);
+  c10::cuda::CUDAGuard guard(seq.device());
+  auto stream = at::cuda::getCurrentCUDAStream();
+  paged::PlanParams p{};
+  p.seq = seq.data_ptr<int>();
+  p.fresh = fresh.data_ptr<int>();
+  p.tables = tables.data_ptr<int>();
+  p.free_pages = free_pages.data_ptr<int>();
+  p.free_head = free_head.data_ptr<int>();
+  p.positions = tok.data_ptr<int>();
+  p.slots = p.positions + n_tokens;
+  p.rows = p.slots + n_tokens;
+  p.ends = req.data_ptr<int>();
+  p.seq_out = p.ends + B;
+  p.head_out = head.data_ptr<int>();
+  p.status = status_ptr(seq.device().index());
+  p.tstride = tables.stride(0);
+  p.B = static_cast<int>(B);
+  p.W = static_cast<int>(tables.size(1));
+  p.N = static_cast<int>(n_tokens);
+  p.n_free = static_cast<int>(free_pages.numel());
+  p.page_shift = paged::shift_of(page_size);
+  const int smem = static_cast<int>(2 * (B + 1) * sizeof(int));
+  if (smem > 48 * 1024) {
+    check_smem_optin(smem, seq.device().index(), "paged_plan");
+    MINT_CUDA_CHECK(cudaFuncSetAttribute(paged::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  }
+  const int64_t work = std::max<int64_t>(n_tokens, B);
+  const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>((work + 1023) / 1024, 1), num_sms(seq.device().index())));
+  paged::plan_kernel<<<grid, paged::kPlanThreads, smem, stream>>>(p);
+  MINT_CUDA_CHECK(cudaGetLastError());
+  count_launch();
+  return {tok.select(0, 0), tok.select(0, 1), tok.select(0, 2), req.select(0, 0), req.select(0, 1), head};
+}
+
+// q [N, Hq, D] normed and rotated; k (normed, rotated) and v stored into the pools' slots. With `dense`
+// also returns k and v as [N, Hkv, D].
+std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, int64_t n_kv, int64_t D,
+                                           const at::Tensor& qs, const at::Tensor& ks,
+                                           const c10::optional<at::Tensor>& cos_t,
+                                           const c10::optional<at::Tensor>& sin_t, const at::Tensor& positions,
+                                           const at::Tensor& slots, at::Tensor& kp, at::Tensor& vp, double eps,
+                                           bool dense) {
+  check_cuda(qkv, "qkv");
+  check_contig(positions, "positions");
+  check_contig(slots, "slots");
+  check_contig(qs, "q_scale");
+  check_contig(ks, "k_scale");
+  const auto dt = qkv.scalar_type();
+  MINT_CHECK((dt == at::kBFloat16 || dt == at::kHalf) && (D == 64 || D == 128 || D == 256),
+             "qk_norm_rope_paged takes bf16 or fp16 heads of 64, 128 or 256");
+  MINT_CHECK(n_q >= 1 && n_kv >= 1 && qkv.dim() == 2 && qkv.size(1) == (n_q + 2 * n_kv) * D, "qkv width mismatch");
+  MINT_CHECK(qkv.stride(1) == 1 && qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+             "qkv rows must be contiguous and 16-byte aligned");
+  const int64_t N = qkv.size(0);
+  MINT_CHECK(positions.scalar_type() == at::kInt && slots.scalar_type() == at::kInt && positions.numel() == N &&
+                 slots.numel() == N,
+             "positions and slots are int32, one per token");
+  MINT_CHECK(qs.scalar_type() == at::kFloat && ks.scalar_type() == at::kFloat && qs.numel() == D && ks.numel() == D,
+             "norm scales are fp32 [head_dim]");
+  paged::check_pool(kp, "k_pages", dt, n_kv, D);
+  paged::check_pool(vp, "v_pages", dt, n_kv, D);
+  MINT_CHECK(kp.sizes() == vp.sizes(), "k_pages and v_pages have different shapes");
+  paged::AppendParams p{};
+  if (cos_t.has_value()) {
+    MINT_CHECK(sin_t.has_value(), "rotation needs both cos and sin");
+    check_contig(*cos_t, "cos");
+    check_contig(*sin_t, "sin");
+    MINT_CHECK(cos_t->scalar_type() == at::kFloat && sin_t->scalar_type() == at::kFloat && cos_t->dim() == 2 &&
+                   cos_t->size(1) == D / 2 && cos_t->sizes() == sin_t->sizes(),
+               "cos / sin are fp32 [positions, head_dim / 2]");
+    p.cos_t = cos_t->data_ptr<float>();
+    p.sin_t = sin_t->data_ptr<float>();
+    p.table_len = static_cast<int>(std::min<int64_t>(cos_t->size(0), INT32_MAX));
+  }
+  auto opts = qkv.options();
+  auto q = at::empty({N, n_q, D}, opts);
+  std::vector<at::Tensor> out{q};
+  if (dense) {
+    out.push_back(at::empty({N, n_kv, D}, opts));
+    out.push_back(at::empty({N, n_kv, D}, opts));
+  }
+  if (N == 0) return out;
+  MINT_CHECK(N * (n_q + 2 * n_kv) * (D / 8) < (1ll << 38), "qk_norm_rope_paged: too many tokens for one call");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  auto stream = at::cuda::getCurrentCUDAStream();
+  p.qkv = qkv.data_ptr();
+  p.qs = qs.data_ptr<float>();
+  p.ks = ks.data_ptr<float>();
+  p.positions = positions.data_ptr<int>();
+  p.slots = slots.data_ptr<int>();
+  p.q = q.data_ptr();
+  p.k = dense ? out[1].data_ptr() : nullptr;
+  p.v = dense ? out[2].data_ptr() : nullptr;
+  p.kp = kp.data_ptr();
+  p.vp = vp.data_ptr();
+  p.status = status_ptr(qkv.device().index());
+  p.qkv_stride = qkv.stride(0);
+  p.kp_page = kp.stride(0);
+  p.kp_head = kp.stride(1);
+  p.kp_line = kp.stride(2);
+  p.vp_page = vp.stride(0);
+  p.vp_head = vp.stride(1);
+  p.vp_line = vp.stride(2);
+  p.N = static_cast<int>(N);
+  p.Hq = static_cast<int>(n_q);
+  p.Hkv = static_cast<int>(n_kv);
+  p.page_shift = paged::shift_of(kp.size(2));
+  p.n_pages = static_cast<int>(kp.size(0));
+  p.eps = static_cast<float>(eps);
+  if (dt == at::kBFloat16) {
+    paged::launch_append<__nv_bfloat16>(p, static_cast<int>(D), stream);
+  } else {
+    paged::launch_append<__half>(p, static_cast<int>(D), stream);
+  }
+  MINT_CUDA_CHECK(cudaGetLastError());
+  count_launch();
+  return out;
+}
+
+}  // namespace mint
