@@ -175,4 +175,25 @@ CUtensorMap make_tmap_4d(const void* base, int dtype, int esize, const uint64_t 
   return map;
 }
 
+CUtensorMap make_tmap_5d(const void* base, int dtype, int esize, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                         const uint32_t (&box)[5], int swizzle) {
+  MINT_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "TMA base address must be 16-byte aligned");
+  CUtensorMap map;
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 5; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+  }
+  for (int i = 0; i < 4; ++i) {
+    MINT_CHECK((strides[i] * esize) % 16 == 0, "TMA strides must be multiples of 16 bytes");
+    st[i] = strides[i] * esize;
+  }
+  CUresult r = encode_fn()(&map, static_cast<CUtensorMapDataType>(dtype), 5, const_cast<void*>(base), d, st, bx, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, static_cast<CUtensorMapSwizzle>(swizzle),
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  MINT_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (5d) failed (", static_cast<int>(r), ")");
+  return map;
+}
+
 }  // namespace mint

@@ -51,6 +51,10 @@ CUtensorMap make_tmap_3d(const void* base, int dtype, int esize, uint64_t d0, ui
 CUtensorMap make_tmap_4d(const void* base, int dtype, int esize, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
                          const uint32_t (&box)[4], int swizzle);
 
+// 5-D tensor map of any dtype: dims (innermost first), strides in elements for dims 1..4.
+CUtensorMap make_tmap_5d(const void* base, int dtype, int esize, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                         const uint32_t (&box)[5], int swizzle);
+
 int num_sms(int device);
 
 // Raise a clear error when a kernel's dynamic shared memory exceeds the device's per-block opt-in
