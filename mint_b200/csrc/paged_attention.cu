@@ -16,12 +16,15 @@
 //   one for V (128-byte swizzle, so the fragment loads are free of bank conflicts) into a ring of stages. Pages
 //   that hold no visible key are requested out of range: TMA fills zeros and reads nothing, and a corrupt
 //   table entry cannot read outside the pool.
-// * Four consumer warps split a tile: RW warps over query rows (16 each), 4 / RW over keys. Each keeps its own
-//   running max, sum and output in registers, so there is no exchange until an item ends, when the warps'
-//   results are merged through the item's last stage. Products run on mma.sync m16n8k16: with at most 16 (64)
-//   live rows an M = 128 tcgen05 tile would be mostly padding, and the tensor pipe is not the bound.
-// * P is split into two 16-bit terms (p = hi + lo) for the second product, so probabilities keep 16 bits of
-//   precision instead of 8 (bf16) at no cost in time; scores, sums and outputs are fp32.
+// * Four consumer warps take 16 keys of a tile each and keep their own running max, sum and output in
+//   registers, so there is no exchange until an item ends, when the warps' results are merged through the
+//   item's last stage. Products run on mma.sync m16n8k16 with the keys (S^T = K Q^T) and the output columns
+//   (O^T = V^T P^T) on the M side and 8 query rows per N block: a group of 1 to 8 query heads fills one block,
+//   where a tcgen05 tile (M = 128 query rows) would be 94 % padding and the tensor pipe is not the bound.
+// * Probabilities are split into two 16-bit terms, p = hi + lo, for the second product: they keep 16 bits of
+//   precision instead of bf16's 8. Groups of at most 4 heads get this for nothing: columns 4-7 of the N block
+//   repeat the rows, carry lo where columns 0-3 carry hi, and are added when the item ends. Scores, sums and
+//   outputs are fp32.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -36,11 +39,12 @@ constexpr int kTile = 64;          // keys per tile
 constexpr int kWarps = 4;          // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kMinTiles = 1;       // a share is at least this many tiles
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinWarps = 8;
 
-template <int D, int RW>
+// NB blocks of 8 query rows per item; TWIN: one block whose columns 4-7 repeat rows 0-3 (hi / lo terms)
+template <int D, int NB>
 struct Config {
-  static constexpr int kRows = 16 * RW;  // query rows per item
+  static constexpr int kRows = 8 * NB;  // query rows per item
   static constexpr int kKvBytes = kTile * D * 2;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kStageBytes = (2 * kKvBytes + kQBytes + 1023) / 1024 * 1024;
@@ -51,7 +55,10 @@ struct Config {
   static constexpr int kFit = ((kTwo ? kHalf : kFull) - kControl) / kStageBytes;
   static constexpr int kStages = kFit < 6 ? kFit : 6;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
+  // the merge goes 16 rows at a time through a stage, lines padded against bank conflicts
+  static constexpr int kMergeRows = kRows < 16 ? kRows : 16, kMergeLine = D + 4;
   static_assert(kStages >= 2 && kSmem + 1024 <= kFull, "shared memory");
+  static_assert(kWarps * kMergeRows * kMergeLine * 4 <= kStageBytes, "merge buffer");
 };
 
 struct TileInfo {  // the tile in a stage, for the consumers
@@ -86,6 +93,13 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
+}
+
+// 8x8 transpose of 16-bit elements spread over a warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 template <typename T>
@@ -156,16 +170,26 @@ __device__ __forceinline__ Span span_at(const AttnParams& p, int n) {
   return span_of(p, p.rows != nullptr ? p.rows[n] : n, p.positions[n]);
 }
 
-template <typename T, int D, int RW>
-__global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
+// CTA c of `ctas` owns tiles [share(c), share(c + 1)) of `all`
+struct Shares {
+  int each, extra;  // the first `extra` CTAs own one tile more
+  __device__ __forceinline__ Shares(int all, int ctas) : each(all / ctas), extra(all - all / ctas * ctas) {}
+  __device__ __forceinline__ int begin(int c) const { return each * c + min(c, extra); }
+  __device__ __forceinline__ int owner(int tile) const {
+    const int big = extra * (each + 1);
+    return tile < big ? tile / (each + 1) : extra + (tile - big) / each;
+  }
+};
+
+template <typename T, int D, int NB, bool TWIN>
+__global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     attend_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, AttnParams p) {
-  using C = Config<D, RW>;
+  using C = Config<D, NB>;
   extern __shared__ uint8_t s_raw[];
   __shared__ uint64_t full[C::kStages], empty[C::kStages], merge;
   __shared__ TileInfo info[C::kStages];
-  __shared__ float2 s_ml[kWarps][16];
-  __shared__ long long s_sum[kWarps + 1], s_off, s_total;
-  __shared__ int s_query, s_abort;
+  __shared__ float2 s_ml[kWarps][C::kRows];
+  __shared__ int s_sum[kWarps + 1], s_query, s_off, s_abort;
   uint8_t* stages = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
   volatile int* abort_flag = &s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -173,6 +197,11 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
   const int per_query = p.Hkv * p.groups;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // this CTA's share of the tiles: totals by a scan over the queries
+  const int chunk = (p.N + kThreads - 1) / kThreads;
+  const int n0 = min(p.N, tid * chunk), n1 = min(p.N, n0 + chunk);
+  int mine = 0;
+  for (int n = n0; n < n1; ++n) mine += span_at(p, n).tiles();
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -180,38 +209,31 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
     }
     mbar_init(&merge, kWarps);
     s_abort = 0;
-    s_query = 0;
-    s_off = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tk);
-    tma_prefetch_desc(&tv);
   }
-  // this CTA's share of the tiles: totals by a scan over the queries
-  const int chunk = (p.N + kThreads - 1) / kThreads;
-  const int n0 = min(p.N, tid * chunk), n1 = min(p.N, n0 + chunk);
-  long long mine = 0;
-  for (int n = n0; n < n1; ++n) mine += span_at(p, n).tiles();
-  long long inc = mine;
+  int inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, inc, d);
+    const int up = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += up;
   }
   if (lane == 31) s_sum[warp] = inc;
   __syncthreads();
-  long long before = inc - mine, total = 0;
+  int before = inc - mine, total = 0;
 #pragma unroll
   for (int w = 0; w <= kWarps; ++w) {
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
   }
-  const long long all = total * per_query;
-  const long long ctas = max(1ll, min(static_cast<long long>(gridDim.x), (all + kMinTiles - 1) / kMinTiles));
-  const long long t0 = cta < ctas ? all * cta / ctas : all, t1 = cta < ctas ? all * (cta + 1) / ctas : all;
-  if (t1 > t0) {
-    const long long u = t0 / per_query;
+  const int all = total * per_query;  // the host keeps it below 2^31
+  const int ctas = max(1, min(static_cast<int>(gridDim.x), (all + kMinTiles - 1) / kMinTiles));
+  const Shares shares(all, ctas);
+  const int t0 = cta < ctas ? shares.begin(cta) : all, t1 = cta < ctas ? shares.begin(cta + 1) : all;
+  const int count = t1 - t0;
+  if (count > 0) {
+    const int u = t0 / per_query;
     if (before <= u && u < before + mine) {
-      long long at = before;
+      int at = before;
       for (int n = n0; n < n1; ++n) {
         const int c = span_at(p, n).tiles();
         if (u < at + c) {
@@ -224,56 +246,80 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
     }
   }
   __syncthreads();
-  const long long count = t1 - t0;
 
   if (warp == kWarps) {
     // ------------------------------------------------------------------------------- producer
-    int n = s_query, stage = 0;
-    long long off = s_off, left = count;
-    uint32_t phase = 0;
-    int4 join = make_int4(0, 0, 0, 0);
-    const int rows_in_box = min(1 << p.page_shift, kTile);
-    const int boxes = kTile / rows_in_box;
-    bool ok = true, bad = false;
-    long long issued = 0;
-    while (left > 0 && ok) {
-      const Span s = span_at(p, n);
-      const int tiles = s.tiles();
-      if (off >= static_cast<long long>(tiles) * per_query) {
-        ++n;
+    struct Piece {  // a run of one item's tiles
+      Span s;
+      int query, group, at, len, tiles;
+    };
+    int query = s_query, off = s_off, left = count;
+    auto next_piece = [&]() {
+      Piece c{};
+      while (left > 0) {
+        c.s = span_at(p, query);
+        c.tiles = c.s.tiles();
+        if (off < c.tiles * per_query) break;
+        ++query;
         off = 0;
-        continue;
       }
-      bad |= p.positions[n] != s.pos;
-      const int group = static_cast<int>(off / tiles), at = static_cast<int>(off - static_cast<long long>(group) * tiles);
-      const int len = static_cast<int>(min(left, static_cast<long long>(tiles - at)));
-      const int kv_head = group / p.groups, row0 = (group - kv_head * p.groups) * C::kRows;
+      if (left > 0) {
+        c.query = query;
+        c.group = off / c.tiles;
+        c.at = off - c.group * c.tiles;
+        c.len = min(left, c.tiles - c.at);
+        off += c.len;
+        left -= c.len;
+      }
+      return c;
+    };
+    // 32 table entries at a time, one per lane; entries of the next run are on their way while one is used
+    auto entries = [&](const Span& s, int page) {
+      return page + lane <= (s.pos >> p.page_shift) ? p.tables[s.row * p.tstride + page + lane] : -1;
+    };
+    auto first_page = [&](const Piece& c) { return ((c.s.first() + c.at) * kTile) >> p.page_shift; };
+    const int box_lines = min(1 << p.page_shift, kTile), boxes = kTile / box_lines;
+    int4 join = make_int4(0, 0, 0, 0);
+    bool ok = true, bad = false;
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    Piece cur = next_piece();
+    int base = 0, entry = -1;
+    if (cur.len > 0) {
+      base = first_page(cur);
+      entry = entries(cur.s, base);
+    }
+    while (cur.len > 0 && ok) {
+      const int rest = left;  // tiles of this CTA after `cur`
+      const Piece nxt = next_piece();
+      int ahead = entries(cur.s, base + 32);
+      const int nxt_base = nxt.len > 0 ? first_page(nxt) : 0;
+      const int nxt_entry = nxt.len > 0 ? entries(nxt.s, nxt_base) : -1;
+      bad |= p.positions[cur.query] != cur.s.pos;
+      const int kv_head = cur.group / p.groups, row0 = (cur.group - kv_head * p.groups) * C::kRows;
       const int live_rows = min(C::kRows, p.G - row0);
       int out = -1;
-      if (at > 0) {
+      if (cur.at > 0) {
         out = 2 * cta;
-      } else if (len < tiles) {
+      } else if (cur.len < cur.tiles) {
         out = 2 * cta + 1;
-        // the last tile's owner: the largest c with all * c / ctas <= tile
-        const long long last = t1 - left + tiles - 1;
-        join = make_int4(n, group, cta, static_cast<int>(((last + 1) * ctas - 1) / all) - cta + 1);
+        join = make_int4(cur.query, cur.group, cta, shares.owner(t1 - rest - cur.len + cur.tiles - 1) - cta + 1);
       }
-      const int* table = p.tables + s.row * p.tstride;
-      const int last_page = s.pos >> p.page_shift;
-      int base = ((s.first() + at) * kTile) >> p.page_shift;
-      int entry = base + lane <= last_page ? table[base + lane] : -1;
-      for (int i = 0; i < len; ++i) {
-        const int key0 = (s.first() + at + i) * kTile;
-        const int page0 = key0 >> p.page_shift;
+      const int last_page = cur.s.pos >> p.page_shift;
+      for (int i = 0; i < cur.len; ++i) {
+        const int key0 = (cur.s.first() + cur.at + i) * kTile;
+        const int page0 = key0 >> p.page_shift, line = key0 & ((1 << p.page_shift) - 1) & -box_lines;
         if (page0 >= base + 32) {
           base = page0;
-          entry = base + lane <= last_page ? table[base + lane] : -1;
+          entry = ahead;
+          ahead = entries(cur.s, base + 32);
         }
-        int page = __shfl_sync(0xffffffffu, entry, (page0 - base + lane) & 31);
-        const int number = page0 + lane;
-        if (number > last_page || ((number + 1) << p.page_shift) <= s.lo) {
-          page = p.n_pages;  // nothing visible in it: zero fill
-        } else if (lane < boxes && (page < 0 || page >= p.n_pages)) {
+        // a page with no visible key is asked for out of range: zeros, no read
+        const int number = base + lane;
+        int page = entry;
+        if (number > last_page || ((number + 1) << p.page_shift) <= cur.s.lo) {
+          page = p.n_pages;
+        } else if (page < 0 || page >= p.n_pages) {
           bad = true;
           page = p.n_pages;
         }
@@ -284,25 +330,26 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
         uint8_t* buf = stages + stage * C::kStageBytes;
         if (lane == 0) {
           TileInfo& t = info[stage];
-          t.query = n;
-          t.group = group;
+          t.query = cur.query;
+          t.group = cur.group;
           t.key0 = key0;
-          t.lo = s.lo;
-          t.hi = s.hi;
-          t.pos = s.pos;
+          t.lo = cur.s.lo;
+          t.hi = cur.s.hi;
+          t.pos = cur.s.pos;
           t.out = out;
-          t.flags = (i == 0 ? 1 : 0) | (i == len - 1 ? 2 : 0);
+          t.flags = (i == 0 ? 1 : 0) | (i == cur.len - 1 ? 2 : 0);
           mbar_arrive_expect_tx(&full[stage], 2 * C::kKvBytes + (i == 0 ? live_rows * D * 2 : 0));
+          if (i == 0)
+            bulk_load(buf + 2 * C::kKvBytes,
+                      static_cast<const T*>(p.q) + (static_cast<long long>(cur.query) * p.Hq + kv_head * p.G + row0) * D,
+                      live_rows * D * 2, &full[stage]);
         }
-        __syncwarp();
-        if (lane < boxes) {
-          const int line = boxes == 1 ? key0 & ((1 << p.page_shift) - 1) : 0;
-          tma_load_page(buf + lane * rows_in_box * D * 2, &tk, &full[stage], line, kv_head, page);
-          tma_load_page(buf + C::kKvBytes + lane * rows_in_box * D * 2, &tv, &full[stage], line, kv_head, page);
-        }
-        if (i == 0 && lane == 0) {
-          const T* q = static_cast<const T*>(p.q) + (static_cast<long long>(n) * p.Hq + kv_head * p.G + row0) * D;
-          bulk_load(buf + 2 * C::kKvBytes, q, live_rows * D * 2, &full[stage]);
+        for (int b = 0; b < boxes; ++b) {
+          const int id = __shfl_sync(0xffffffffu, page, page0 - base + b);
+          if (lane == 0) {
+            tma_load_page(buf + b * box_lines * D * 2, &tk, &full[stage], line, kv_head, id);
+            tma_load_page(buf + C::kKvBytes + b * box_lines * D * 2, &tv, &full[stage], line, kv_head, id);
+          }
         }
         ++issued;
         if (++stage == C::kStages) {
@@ -310,8 +357,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
           phase ^= 1u;
         }
       }
-      off += len;
-      left -= len;
+      cur = nxt;
+      base = nxt_base;
+      entry = nxt_entry;
     }
     if (lane == 0) p.joins[cta] = join;
     if (__any_sync(0xffffffffu, bad) && lane == 0) record_status(p.status, kStatusBadArgument);
@@ -332,217 +380,232 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
     uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + static_cast<long long>(n) * p.Hq * D);
     for (int i = tid; i < p.Hq * D / 8; i += 32 * kWarps) o[i] = make_uint4(0, 0, 0, 0);
   }
-  const int rw = warp % RW, kw = warp / RW;
-  const int box_shift = min(p.page_shift, 6), box_rows = 1 << box_shift;
-  const uint32_t half_stride = box_rows * 128;  // bytes between 64-column parts of a box
-  auto line_offset = [&](int r) { return static_cast<uint32_t>((r >> box_shift) * box_rows * D * 2 + (r & (box_rows - 1)) * 128); };
-  uint32_t k_line[RW], v_line[RW];
-#pragma unroll
-  for (int b = 0; b < RW; ++b) {
-    const int r0 = (kw * RW + b) * 16;
-    k_line[b] = line_offset(r0 + (lane & 7) + ((lane >> 4) << 3));
-    v_line[b] = line_offset(r0 + (lane & 15));
-  }
-  const uint32_t k_chunk = ((lane >> 3) & 1) ^ (lane & 7), v_chunk = (lane >> 4) ^ (lane & 7);
+  // tile line r: 64-column parts of a box are half_stride bytes apart, 16-byte chunk c of a line sits at c ^ (r & 7)
+  const int box_shift = min(p.page_shift, 6), box_lines = 1 << box_shift;
+  const uint32_t half_stride = box_lines * 128;
+  auto line_offset = [&](int r) { return static_cast<uint32_t>((r >> box_shift) * box_lines * D * 2 + (r & (box_lines - 1)) * 128); };
+  const uint32_t k_line = line_offset(warp * 16 + (lane & 15));
+  const uint32_t v_line = line_offset(warp * 16 + (lane & 7) + ((lane >> 4) << 3));
+  const uint32_t k_chunk = (lane >> 4) ^ (lane & 7), v_chunk = ((lane >> 3) & 1) ^ (lane & 7);
   const uint32_t base_addr = smem_u32(stages);
+  const int my_key = warp * 16 + (lane >> 2);  // and + 8
+  const int my_row = 2 * (lane & 3);           // and + 1, in each block of 8
 
-  uint32_t qf[D / 16][4];
-  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope[2] = {0.f, 0.f};
+  uint32_t qf[NB][D / 16][2];
+  float o[NB][D / 16][4], m[NB][2], l[NB][2], slope[NB][2];
   int stage = 0;
   uint32_t phase = 0, merge_phase = 0;
-  for (long long it = 0; it < count; ++it) {
+  for (int it = 0; it < count; ++it) {
     if (!mbar_wait_warp(&full[stage], phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
     const TileInfo t = info[stage];
     const uint32_t k_addr = base_addr + stage * C::kStageBytes, v_addr = k_addr + C::kKvBytes;
-    const int kv_head = t.group / p.groups, row0 = (t.group - kv_head * p.groups) * C::kRows;
     if (t.flags & 1) {
-      const uint32_t q_addr = k_addr + 2 * C::kKvBytes + (rw * 16 + (lane & 15)) * (D * 2) + (lane >> 4) * 16;
+      const int kv_head = t.group / p.groups, row0 = (t.group - kv_head * p.groups) * C::kRows;
+      const int live_rows = min(C::kRows, p.G - row0);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) ldsm4(qf[ks], q_addr + ks * 32);
+      for (int nb = 0; nb < NB; ++nb) {
+        // rows past the last repeat it: they cost nothing and are not written
+        const int row = min(TWIN ? lane & 3 : nb * 8 + (lane & 7), live_rows - 1);
+        const uint32_t q_addr = k_addr + 2 * C::kKvBytes + row * (D * 2) + (lane >> 3) * 16;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int ks = 0; ks < D / 32; ++ks) {
+          uint32_t r[4];
+          ldsm4(r, q_addr + ks * 64);
+          qf[nb][2 * ks][0] = r[0];
+          qf[nb][2 * ks][1] = r[1];
+          qf[nb][2 * ks + 1][0] = r[2];
+          qf[nb][2 * ks + 1][1] = r[3];
+        }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-        if (p.slopes != nullptr) {
-          const int row = row0 + rw * 16 + r * 8 + (lane >> 2);
-          slope[r] = row < p.G ? p.slopes[kv_head * p.G + row] * 1.4426950408889634f : 0.f;
+        for (int i = 0; i < D / 16; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          m[nb][c] = -INFINITY;
+          l[nb][c] = 0.f;
+          const int r = min(TWIN ? (my_row + c) & 3 : nb * 8 + my_row + c, live_rows - 1);
+          slope[nb][c] = p.slopes != nullptr ? p.slopes[kv_head * p.G + row0 + r] * 1.4426950408889634f : 0.f;
         }
       }
     }
-    // S = Q K^T
-    float s[2 * RW][4];
+    // S^T = K Q^T: s[nb][0..1] = key my_key, rows my_row, + 1; s[nb][2..3] = key my_key + 8
+    float s[NB][4];
+    {
+      float alt[NB][4];  // second chain of accumulators: halves the dependent products
 #pragma unroll
-    for (int b = 0; b < RW; ++b) {
-      float alt[2][4];  // second chain of accumulators: halves the dependent products
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[2 * b][e] = s[2 * b + 1][e] = alt[0][e] = alt[1][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[nb][e] = alt[nb][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         uint32_t kf[4];
-        ldsm4(kf, k_addr + k_line[b] + (ks / 4) * half_stride + (((ks % 4) * 2) ^ k_chunk) * 16);
-        if (ks & 1) {
-          mma16816<T>(alt[0], qf[ks], kf[0], kf[1]);
-          mma16816<T>(alt[1], qf[ks], kf[2], kf[3]);
-        } else {
-          mma16816<T>(s[2 * b], qf[ks], kf[0], kf[1]);
-          mma16816<T>(s[2 * b + 1], qf[ks], kf[2], kf[3]);
-        }
+        ldsm4(kf, k_addr + k_line + (ks / 4) * half_stride + (((ks % 4) * 2) ^ k_chunk) * 16);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma16816<T>((ks & 1) ? alt[nb] : s[nb], kf, qf[nb][ks][0], qf[nb][ks][1]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[2 * b][e] = (s[2 * b][e] + alt[0][e]) * p.scale_log2;
-        s[2 * b + 1][e] = (s[2 * b + 1][e] + alt[1][e]) * p.scale_log2;
-      }
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nb][e] = (s[nb][e] + alt[nb][e]) * p.scale_log2;
     }
-    const int key_base = t.key0 + kw * RW * 16 + 2 * (lane & 3);
     if (p.slopes != nullptr) {
 #pragma unroll
-      for (int b = 0; b < 2 * RW; ++b)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          s[b][e] = fmaf(slope[e >> 1], static_cast<float>(key_base + b * 8 + (e & 1) - t.pos), s[b][e]);
+          s[nb][e] = fmaf(slope[nb][e & 1], static_cast<float>(t.key0 + my_key + (e >> 1) * 8 - t.pos), s[nb][e]);
     }
     const bool edge = t.key0 < t.lo || t.key0 + kTile > t.hi;
     if (edge) {
 #pragma unroll
-      for (int b = 0; b < 2 * RW; ++b)
+      for (int e = 0; e < 4; e += 2) {
+        const int key = t.key0 + my_key + e * 4;
+        if (key < t.lo || key >= t.hi) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key_base + b * 8 + (e & 1);
-          if (key < t.lo || key >= t.hi) s[b][e] = -INFINITY;
+          for (int nb = 0; nb < NB; ++nb) s[nb][e] = s[nb][e + 1] = -INFINITY;
         }
+      }
       // a line outside the keys seen may hold anything (0 * NaN is NaN): clear the V lines this warp reads
-#pragma unroll
-      for (int b = 0; b < RW; ++b) {
-        const int r0 = (kw * RW + b) * 16;
-        for (int i = lane; i < 16 * (D / 8); i += 32) {
-          const int r = r0 + i / (D / 8), c = i % (D / 8);
-          const int key = t.key0 + r;
-          if (key < t.lo || key >= t.hi)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_addr + line_offset(r) + (c / 8) * half_stride +
-                                                                         (c % 8) * 16),
-                         "r"(0)
-                         : "memory");
-        }
+      for (int i = lane; i < 16 * (D / 8); i += 32) {
+        const int r = warp * 16 + i / (D / 8), c = i % (D / 8);
+        if (t.key0 + r < t.lo || t.key0 + r >= t.hi)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_addr + line_offset(r) + (c / 8) * half_stride +
+                                                                       (c % 8) * 16),
+                       "r"(0)
+                       : "memory");
       }
       __syncwarp();
     }
-    // running max and rescale
-    float base[2];
+    // running max over the keys (lanes 4 apart hold a row's keys) and rescale
+    float fix[NB][2];
     bool moved = false;
-    float fix[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = -INFINITY;
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int b = 0; b < 2 * RW; ++b) mx = fmaxf(mx, fmaxf(s[b][2 * r], s[b][2 * r + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float next = fmaxf(m[r], mx);
-      base[r] = next == -INFINITY ? 0.f : next;
-      fix[r] = exp2f(m[r] - base[r]);
-      moved |= next != m[r];
-      m[r] = next;
-      l[r] *= fix[r];
-    }
+      for (int c = 0; c < 2; ++c) {
+        float mx = fmaxf(s[nb][c], s[nb][2 + c]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float next = fmaxf(m[nb][c], mx);
+        const float base = next == -INFINITY ? 0.f : next;
+        fix[nb][c] = exp2f(m[nb][c] - base);
+        moved |= next != m[nb][c];
+        m[nb][c] = next;
+        s[nb][c] = exp2f(s[nb][c] - base);
+        s[nb][2 + c] = exp2f(s[nb][2 + c] - base);
+        l[nb][c] = fmaf(l[nb][c], fix[nb][c], s[nb][c] + s[nb][2 + c]);
+      }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= fix[0];
-        o[i][1] *= fix[0];
-        o[i][2] *= fix[1];
-        o[i][3] *= fix[1];
-      }
-    }
-    // O += P V
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int b = 0; b < RW; ++b) {
-      uint32_t hi[4], lo[4];
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nb][i][e] *= fix[nb][e & 1];
+    }
+    // O^T += V^T P^T; P^T's operand layout is the transpose of S^T's
+    uint32_t hi[NB][2], lo[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float* x = s[2 * b + h];
-        x[0] = exp2f(x[0] - base[0]);
-        x[1] = exp2f(x[1] - base[0]);
-        x[2] = exp2f(x[2] - base[1]);
-        x[3] = exp2f(x[3] - base[1]);
-        l[0] += x[0] + x[1];
-        l[1] += x[2] + x[3];
-        split2<T>(x[0], x[1], hi[2 * h], lo[2 * h]);
-        split2<T>(x[2], x[3], hi[2 * h + 1], lo[2 * h + 1]);
+        uint32_t a, b;
+        split2<T>(s[nb][2 * h], s[nb][2 * h + 1], a, b);
+        if (TWIN) {
+          hi[nb][h] = transpose8((lane & 2) ? b : a);  // columns 4-7 carry lo
+        } else {
+          hi[nb][h] = transpose8(a);
+          lo[nb][h] = transpose8(b);
+        }
       }
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd) {
-        uint32_t vf[4];
-        ldsm4_t(vf, v_addr + v_line[b] + (dd / 4) * half_stride + (((dd % 4) * 2) ^ v_chunk) * 16);
-        mma16816<T>(o[2 * dd], hi, vf[0], vf[1]);
-        mma16816<T>(o[2 * dd + 1], hi, vf[2], vf[3]);
-        mma16816<T>(o[2 * dd], lo, vf[0], vf[1]);
-        mma16816<T>(o[2 * dd + 1], lo, vf[2], vf[3]);
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t vf[4];
+      ldsm4_t(vf, v_addr + v_line + (i / 4) * half_stride + (((i % 4) * 2) ^ v_chunk) * 16);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        mma16816<T>(o[nb][i], vf, hi[nb][0], hi[nb][1]);
+        if (!TWIN) mma16816<T>(o[nb][i], vf, lo[nb][0], lo[nb][1]);
       }
     }
     if (t.flags & 2) {
-      // merge the warps' results through this stage's K and V (4 warps * 16 rows * D floats fill them exactly)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&merge);  // done with this stage, and with the previous item's s_ml
-      if (!mbar_wait_warp(&merge, merge_phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
-      merge_phase ^= 1u;
+      // merge the warps' results through this stage, 16 rows at a time
+      const int kv_head = t.group / p.groups, row0 = (t.group - kv_head * p.groups) * C::kRows;
+      const int live_rows = min(C::kRows, p.G - row0);
       float* buf = reinterpret_cast<float*>(stages + stage * C::kStageBytes);
-      const int rows_live = min(C::kRows, p.G - row0);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = r * 8 + (lane >> 2);
-        if ((lane & 3) == 0) s_ml[warp][row] = make_float2(m[r], l[r]);
-        if (rw * 16 + row < rows_live) {
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<float2*>(buf + (warp * 16 + row) * D + ((i * 8 + 2 * (lane & 3)) ^ ((row & 7) * 8))) =
-                make_float2(o[i][2 * r], o[i][2 * r + 1]);
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
         }
+      if (TWIN) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[0][i][e] += __shfl_xor_sync(0xffffffffu, o[0][i][e], 2);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&merge);
-      if (!mbar_wait_warp(&merge, merge_phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
-      merge_phase ^= 1u;
-      for (int i = tid; i < rows_live * (D / 4); i += 32 * kWarps) {
-        const int row = i / (D / 4), c = (i % (D / 4)) * 4;
-        const int rg = row / 16, rr = row % 16;
-        float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps / RW; ++w) M = fmaxf(M, s_ml[w * RW + rg][rr].x);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int mr = 0; mr < C::kRows; mr += C::kMergeRows) {
+        if (mr >= live_rows) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&merge);  // done with this stage, and with what was merged before
+        if (!mbar_wait_warp(&merge, merge_phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
+        merge_phase ^= 1u;
 #pragma unroll
-        for (int w = 0; w < kWarps / RW; ++w) {
-          const float2 ml = s_ml[w * RW + rg][rr];
-          const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-          const float4 y = *reinterpret_cast<const float4*>(buf + ((w * RW + rg) * 16 + rr) * D + (c ^ ((rr & 7) * 8)));
-          L = fmaf(ml.y, f, L);
-          x.x = fmaf(y.x, f, x.x);
-          x.y = fmaf(y.y, f, x.y);
-          x.z = fmaf(y.z, f, x.z);
-          x.w = fmaf(y.w, f, x.w);
-        }
-        if (t.out < 0) {
-          const float inv = 1.f / L;
-          T* dst = static_cast<T*>(p.o) + (static_cast<long long>(t.query) * p.Hq + kv_head * p.G + row0 + row) * D + c;
-          T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
-          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
-        } else {
-          const long long at = static_cast<long long>(t.out) * p.part_rows + row;
-          *reinterpret_cast<float4*>(p.part_o + at * D + c) = x;
-          if (c == 0) p.part_ml[at] = make_float2(M, L);
+        for (int nb = mr / 8; nb < (mr + C::kMergeRows) / 8; ++nb)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int row = nb * 8 + my_row + c;
+            if (row < live_rows) {
+              if (lane < 4) s_ml[warp][row] = make_float2(m[nb][c], l[nb][c]);
+              float* dst = buf + (warp * C::kMergeRows + row - mr) * C::kMergeLine + (lane >> 2);
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                dst[i * 16] = o[nb][i][c];
+                dst[i * 16 + 8] = o[nb][i][2 + c];
+              }
+            }
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&merge);
+        if (!mbar_wait_warp(&merge, merge_phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
+        merge_phase ^= 1u;
+        const int rows_here = min(C::kMergeRows, live_rows - mr);
+        for (int i = tid; i < rows_here * (D / 4); i += 32 * kWarps) {
+          const int r = i / (D / 4), row = mr + r, c = (i % (D / 4)) * 4;
+          float M = -INFINITY, L = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w][row].x);
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = s_ml[w][row];
+            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+            const float4 y = *reinterpret_cast<const float4*>(buf + (w * C::kMergeRows + r) * C::kMergeLine + c);
+            L = fmaf(ml.y, f, L);
+            x.x = fmaf(y.x, f, x.x);
+            x.y = fmaf(y.y, f, x.y);
+            x.z = fmaf(y.z, f, x.z);
+            x.w = fmaf(y.w, f, x.w);
+          }
+          if (t.out < 0) {
+            const float inv = 1.f / L;
+            T* dst = static_cast<T*>(p.o) + (static_cast<long long>(t.query) * p.Hq + kv_head * p.G + row0 + row) * D + c;
+            T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+          } else {
+            const long long at = static_cast<long long>(t.out) * p.part_rows + row;
+            *reinterpret_cast<float4*>(p.part_o + at * D + c) = x;
+            if (c == 0) p.part_ml[at] = make_float2(M, L);
+          }
         }
       }
       __syncwarp();
     }
     // plain stores to the stage come before the next copy into it
     if (edge || (t.flags & 2)) fence_proxy_async_smem();
+    __syncwarp();
     if (lane == 0) mbar_arrive(&empty[stage]);
     if (++stage == C::kStages) {
       stage = 0;
@@ -551,12 +614,12 @@ __global__ void __launch_bounds__(kThreads, Config<D, RW>::kTwo ? 2 : 1)
   }
 }
 
-// Joins the partials of the item that CTA blockIdx.x began and did not finish: partial 0 in slot 2c + 1, the
-// following CTAs' in slot 2c'. Warps take (row, every S-th partial); the S sums of a row are added in order.
+// Joins the partials of the item that CTA blockIdx.x began and did not finish: the first in slot 2c + 1, the
+// following CTAs' in slots 2c'. A block takes every gridDim.y-th row; its warps take every 8th partial, and
+// the warps' sums are added in order.
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p) {
   constexpr int E = D / 32;
-  constexpr int kJoinWarps = kJoinThreads / 32;
   __shared__ float s_x[kJoinWarps][D];
   __shared__ float2 s_ml[kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -565,50 +628,41 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(AttnParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kv_head = join.y / p.groups, row0 = (join.y - kv_head * p.groups) * p.part_rows;
   const int rows = min(p.part_rows, p.G - row0);
-  int together = 1;  // rows in flight: a power of two up to the warps
-  while (together < rows && together < kJoinWarps) together *= 2;
-  const int splits = kJoinWarps / together;
-  const int slot0 = warp / together;
-  for (int r0 = 0; r0 < rows; r0 += together) {
-    const int row = r0 + warp % together;
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
     float M = -INFINITY, L = 0.f, x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = 0.f;
-    if (row < rows) {
 #pragma unroll 4
-      for (int i = slot0; i < join.w; i += splits) {
-        const long long at = static_cast<long long>(i == 0 ? 2 * join.z + 1 : 2 * (join.z + i)) * p.part_rows + row;
-        const float2 ml = p.part_ml[at];
-        float y[E];
+    for (int i = warp; i < join.w; i += kJoinWarps) {
+      const long long at = static_cast<long long>(i == 0 ? 2 * join.z + 1 : 2 * (join.z + i)) * p.part_rows + row;
+      const float2 ml = p.part_ml[at];
+      float y[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = p.part_o[at * D + e * 32 + lane];
-        const float next = fmaxf(M, ml.x), base = next == -INFINITY ? 0.f : next;
-        const float f = exp2f(M - base), g = exp2f(ml.x - base);
-        M = next;
-        L = L * f + ml.y * g;
+      for (int e = 0; e < E; ++e) y[e] = p.part_o[at * D + e * 32 + lane];
+      const float next = fmaxf(M, ml.x), base = next == -INFINITY ? 0.f : next;
+      const float f = exp2f(M - base), g = exp2f(ml.x - base);
+      M = next;
+      L = L * f + ml.y * g;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = fmaf(y[e], g, x[e] * f);
-      }
+      for (int e = 0; e < E; ++e) x[e] = fmaf(y[e], g, x[e] * f);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) s_x[warp][e * 32 + lane] = x[e];
     if (lane == 0) s_ml[warp] = make_float2(M, L);
     __syncthreads();
-    if (warp < together && row < rows) {
-      float top = -INFINITY, sum = 0.f, y[E];
-      for (int s = 0; s < splits; ++s) top = fmaxf(top, s_ml[s * together + warp].x);
+    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+      float top = -INFINITY, sum = 0.f, y = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = 0.f;
-      for (int s = 0; s < splits; ++s) {
-        const float2 ml = s_ml[s * together + warp];
+      for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float2 ml = s_ml[w];
         const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
         sum = fmaf(ml.y, f, sum);
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = fmaf(s_x[s * together + warp][e * 32 + lane], f, y[e]);
+        y = fmaf(s_x[w][d], f, y);
       }
-      T* dst = static_cast<T*>(p.o) + (static_cast<long long>(join.x) * p.Hq + kv_head * p.G + row0 + row) * D;
-#pragma unroll
-      for (int e = 0; e < E; ++e) dst[e * 32 + lane] = from_f32<T>(y[e] / sum);
+      static_cast<T*>(p.o)[(static_cast<long long>(join.x) * p.Hq + kv_head * p.G + row0 + row) * D + d] =
+          from_f32<T>(y / sum);
     }
     __syncthreads();
   }
@@ -625,61 +679,80 @@ CUtensorMap page_map(const at::Tensor& t, int dtype) {
   return make_tmap_5d(t.data_ptr(), dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int D, int RW>
-void launch_attend(AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& q, bool may_split,
-                   cudaStream_t stream) {
-  using C = Config<D, RW>;
+template <typename T, int D, int NB, bool TWIN>
+void launch_attend(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& q, bool may_split,
+                   int64_t tiles_bound, cudaStream_t stream) {
+  using C = Config<D, NB>;
   const int device = q.device().index();
-  const auto kernel = attend_kernel<T, D, RW>;
+  const auto kernel = attend_kernel<T, D, NB, TWIN>;
   check_smem_optin(C::kSmem, device, "paged_attention");
   MINT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   const int grid = num_sms(device) * (C::kTwo ? 2 : 1);
   p.groups = (p.G + C::kRows - 1) / C::kRows;
-  p.part_rows = p.groups > 1 ? C::kRows : std::min(p.G, C::kRows);
+  p.part_rows = p.groups > 1 ? C::kRows : p.G;
   const int64_t slots = 2ll * grid * p.part_rows;
   auto ws = at::empty({slots * (D + 2) + 4 * grid}, q.options().dtype(at::kFloat));
   p.part_o = ws.data_ptr<float>();
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * D);
   p.joins = reinterpret_cast<int4*>(p.part_o + slots * (D + 2));
-  kernel<<<grid, kThreads, C::kSmem, stream>>>(tk, tv, p);
-  MINT_CUDA_CHECK(cudaGetLastError());
-  count_launch();
-  if (!may_split) return;
-  // launched while the first kernel still runs; it waits for that kernel's end on the device
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  MINT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p));
-  count_launch();
-}
-
-template <typename T, int D>
-void dispatch_rows(AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& q, bool may_split,
-                   cudaStream_t stream) {
-  if (p.G <= 16) {
-    launch_attend<T, D, 1>(p, tk, tv, q, may_split, stream);
-  } else if (p.G <= 32) {
-    launch_attend<T, D, 2>(p, tk, tv, q, may_split, stream);
-  } else {
-    launch_attend<T, D, 4>(p, tk, tv, q, may_split, stream);
+  // tile numbers are ints: so many queries that they might not fit go in several launches
+  const int64_t per_query = tiles_bound * p.Hkv * p.groups;
+  MINT_CHECK(per_query <= INT_MAX, "paged_attention: a query may have too many tiles");
+  const int step = static_cast<int>(std::min<int64_t>(p.N, INT_MAX / per_query));
+  const AttnParams all = p;
+  for (int n = 0; n < all.N; n += step) {
+    p.N = std::min(step, all.N - n);
+    p.q = static_cast<const T*>(all.q) + static_cast<int64_t>(n) * p.Hq * D;
+    p.o = static_cast<T*>(all.o) + static_cast<int64_t>(n) * p.Hq * D;
+    p.positions = all.positions + n;
+    if (all.rows != nullptr) {
+      p.rows = all.rows + n;
+    } else {
+      p.tables = all.tables + n * all.tstride;
+      p.B = p.N;
+    }
+    kernel<<<grid, kThreads, C::kSmem, stream>>>(tk, tv, p);
+    MINT_CUDA_CHECK(cudaGetLastError());
+    count_launch();
+    if (!may_split) continue;
+    // launched while the first kernel still runs; it waits for that kernel's end on the device
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, std::min(p.part_rows, 4));
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    MINT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p));
+    count_launch();
   }
 }
 
-template <typename T>
-void dispatch_dim(AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, const at::Tensor& q, bool may_split,
-                  cudaStream_t stream) {
-  if (q.size(2) == 64) {
-    dispatch_rows<T, 64>(p, tk, tv, q, may_split, stream);
-  } else if (q.size(2) == 128) {
-    dispatch_rows<T, 128>(p, tk, tv, q, may_split, stream);
+// Query rows per item: 4 (hi and lo terms side by side in one block of 8), 8, 16 or, where the outputs fit
+// the registers (heads up to 128), 32. Wider groups are several items, which read K and V again (from L2).
+template <typename T, int D, typename... Args>
+void dispatch_rows(const AttnParams& p, Args&&... args) {
+  if (p.G <= 4) {
+    launch_attend<T, D, 1, true>(p, args...);
+  } else if (p.G <= 8) {
+    launch_attend<T, D, 1, false>(p, args...);
+  } else if (p.G <= 16 || D == 256) {
+    launch_attend<T, D, 2, false>(p, args...);
   } else {
-    dispatch_rows<T, 256>(p, tk, tv, q, may_split, stream);
+    launch_attend<T, D, D == 256 ? 2 : 4, false>(p, args...);
+  }
+}
+
+template <typename T, typename... Args>
+void dispatch_dim(const AttnParams& p, int64_t D, Args&&... args) {
+  if (D == 64) {
+    dispatch_rows<T, 64>(p, args...);
+  } else if (D == 128) {
+    dispatch_rows<T, 128>(p, args...);
+  } else {
+    dispatch_rows<T, 256>(p, args...);
   }
 }
 
@@ -746,12 +819,14 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   const int type = dt == at::kBFloat16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUtensorMap tk = paged::page_map(kp, type), tv = paged::page_map(vp, type);
-  // one tile at most per item: nothing to join
-  const bool may_split = tables.size(1) * kp.size(2) > paged::kTile;
+  // the most tiles that a query can have; with one at most there is nothing to join
+  int64_t tiles_bound = std::max<int64_t>(1, (tables.size(1) * kp.size(2) + paged::kTile - 1) / paged::kTile);
+  if (window >= 0) tiles_bound = std::min<int64_t>(tiles_bound, window / paged::kTile + 2);
+  const bool may_split = tiles_bound > 1;
   if (dt == at::kBFloat16) {
-    paged::dispatch_dim<__nv_bfloat16>(p, tk, tv, q, may_split, stream);
+    paged::dispatch_dim<__nv_bfloat16>(p, D, tk, tv, q, may_split, tiles_bound, stream);
   } else {
-    paged::dispatch_dim<__half>(p, tk, tv, q, may_split, stream);
+    paged::dispatch_dim<__half>(p, D, tk, tv, q, may_split, tiles_bound, stream);
   }
   return o;
 }
