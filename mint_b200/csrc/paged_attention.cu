@@ -12,10 +12,11 @@
 //   CUDA graph follows the lengths). A CTA whose share starts or ends inside an item leaves an fp32 partial
 //   (running max, sum, unnormalized output); a second, small kernel joins an item's partials in tile order,
 //   so results do not depend on timing.
-// * One producer warp reads the block table 32 entries at a time and issues one TMA box per page for K and
-//   one for V (128-byte swizzle, so the fragment loads are free of bank conflicts) into a ring of stages. Pages
-//   that hold no visible key are requested out of range: TMA fills zeros and reads nothing, and a corrupt
-//   table entry cannot read outside the pool.
+// * Two producer warps, one for K and one for V (a thread issues a box every ~90 cycles, and a tile has 8 boxes
+//   of 16 lines each), read the block table 32 entries at a time and issue one TMA box per page (128-byte
+//   swizzle, so the fragment loads are free of bank conflicts) into a ring of stages. Pages that hold no
+//   visible key are requested out of range: TMA fills zeros and reads nothing, and a corrupt table entry
+//   cannot read outside the pool.
 // * Four consumer warps take 16 keys of a tile each and keep their own running max, sum and output in
 //   registers, so there is no exchange until an item ends, when the warps' results are merged through the
 //   item's last stage. Products run on mma.sync m16n8k16 with the keys (S^T = K Q^T) and the output columns
@@ -37,7 +38,7 @@ namespace paged {
 
 constexpr int kTile = 64;          // keys per tile
 constexpr int kWarps = 4;          // consumer warps
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kThreads = 32 * (kWarps + 2);  // and a producer warp each for K and V
 constexpr int kMinTiles = 1;       // a share is at least this many tiles
 constexpr int kJoinWarps = 8;
 
@@ -49,7 +50,7 @@ struct Config {
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kStageBytes = (2 * kKvBytes + kQBytes + 1023) / 1024 * 1024;
   // two CTAs per SM where three stages fit twice, else one
-  static constexpr int kControl = 2048;  // barriers, tile descriptions, merge statistics, base alignment
+  static constexpr int kControl = 3072;  // scan, barriers, tile descriptions, merge statistics, base alignment
   static constexpr int kHalf = 113 * 1024, kFull = 227 * 1024;
   static constexpr bool kTwo = (kHalf - kControl) / kStageBytes >= 3;
   static constexpr int kFit = ((kTwo ? kHalf : kFull) - kControl) / kStageBytes;
@@ -181,6 +182,16 @@ struct Shares {
   }
 };
 
+// mbar_wait_warp that polls a while before it reads the clock and the wait limit (a global load, as long as
+// the whole wait for a tile)
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t* status, volatile int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  for (int i = 0; i < 64; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(addr, parity))) return true;
+  }
+  return mbar_wait_warp(bar, parity, status, kStatusTimeoutAttention, abort_flag);
+}
+
 template <typename T, int D, int NB, bool TWIN>
 __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     attend_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, AttnParams p) {
@@ -189,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
   __shared__ uint64_t full[C::kStages], empty[C::kStages], merge;
   __shared__ TileInfo info[C::kStages];
   __shared__ float2 s_ml[kWarps][C::kRows];
-  __shared__ int s_sum[kWarps + 1], s_query, s_off, s_abort;
+  __shared__ int s_inc[kThreads], s_sum[kThreads / 32], s_abort;
   uint8_t* stages = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
   volatile int* abort_flag = &s_abort;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -197,63 +208,74 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
   const int per_query = p.Hkv * p.groups;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // this CTA's share of the tiles: totals by a scan over the queries
+  // this CTA's share of the tiles: totals by a scan over the queries, `chunk` of them per thread
   const int chunk = (p.N + kThreads - 1) / kThreads;
   const int n0 = min(p.N, tid * chunk), n1 = min(p.N, n0 + chunk);
-  int mine = 0;
-  for (int n = n0; n < n1; ++n) mine += span_at(p, n).tiles();
+  int inc = 0;
+  for (int n = n0; n < n1; ++n) inc += span_at(p, n).tiles();
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 2);
       mbar_init(&empty[i], kWarps);
     }
     mbar_init(&merge, kWarps);
     s_abort = 0;
     fence_mbar_init();
   }
-  int inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += up;
   }
+  s_inc[tid] = inc;
   if (lane == 31) s_sum[warp] = inc;
   __syncthreads();
-  int before = inc - mine, total = 0;
+  int total = 0;
 #pragma unroll
-  for (int w = 0; w <= kWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
+  for (int w = 0; w < kThreads / 32; ++w) total += s_sum[w];
   const int all = total * per_query;  // the host keeps it below 2^31
   const int ctas = max(1, min(static_cast<int>(gridDim.x), (all + kMinTiles - 1) / kMinTiles));
   const Shares shares(all, ctas);
   const int t0 = cta < ctas ? shares.begin(cta) : all, t1 = cta < ctas ? shares.begin(cta + 1) : all;
   const int count = t1 - t0;
-  if (count > 0) {
-    const int u = t0 / per_query;
-    if (before <= u && u < before + mine) {
-      int at = before;
-      for (int n = n0; n < n1; ++n) {
-        const int c = span_at(p, n).tiles();
-        if (u < at + c) {
-          s_query = n;
-          s_off = t0 - at * per_query;
-          break;
-        }
-        at += c;
-      }
-    }
-  }
-  __syncthreads();
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------------------------- producer
+  if (warp >= kWarps) {
+    // ------------------------------------------------------------------------------ producers
+    const bool is_k = warp == kWarps;
+    int query = 0, off = 0, left = count;
+    if (count > 0) {  // the share's first query: the chunk that holds tile t0, then the query in it
+      const int u = t0 / per_query;
+      int sum = 0, at = 0, owner = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        const int end = sum + s_inc[w * 32 + lane];
+        const unsigned past = __ballot_sync(0xffffffffu, end <= u);
+        owner += __popc(past);
+        if (past != 0) at = __shfl_sync(0xffffffffu, end, 31 - __clz(past));
+        sum += s_sum[w];
+      }
+      query = owner * chunk;
+      if (chunk > 1) {
+        while (true) {
+          int end = query + lane < p.N ? span_at(p, query + lane).tiles() : 0;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, end, d);
+            if (lane >= d) end += up;
+          }
+          end += at;
+          const unsigned past = __ballot_sync(0xffffffffu, end <= u);
+          if (past != 0) at = __shfl_sync(0xffffffffu, end, 31 - __clz(past));
+          query += __popc(past);
+          if (past != 0xffffffffu) break;
+        }
+      }
+      off = t0 - at * per_query;
+    }
     struct Piece {  // a run of one item's tiles
       Span s;
       int query, group, at, len, tiles;
     };
-    int query = s_query, off = s_off, left = count;
     auto next_piece = [&]() {
       Piece c{};
       while (left > 0) {
@@ -279,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     };
     auto first_page = [&](const Piece& c) { return ((c.s.first() + c.at) * kTile) >> p.page_shift; };
     const int box_lines = min(1 << p.page_shift, kTile), boxes = kTile / box_lines;
+    const CUtensorMap* map = is_k ? &tk : &tv;
     int4 join = make_int4(0, 0, 0, 0);
     bool ok = true, bad = false;
     int stage = 0, issued = 0;
@@ -291,11 +314,6 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     }
     while (cur.len > 0 && ok) {
       const int rest = left;  // tiles of this CTA after `cur`
-      const Piece nxt = next_piece();
-      int ahead = entries(cur.s, base + 32);
-      const int nxt_base = nxt.len > 0 ? first_page(nxt) : 0;
-      const int nxt_entry = nxt.len > 0 ? entries(nxt.s, nxt_base) : -1;
-      bad |= p.positions[cur.query] != cur.s.pos;
       const int kv_head = cur.group / p.groups, row0 = (cur.group - kv_head * p.groups) * C::kRows;
       const int live_rows = min(C::kRows, p.G - row0);
       int out = -1;
@@ -306,6 +324,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
         join = make_int4(cur.query, cur.group, cta, shares.owner(t1 - rest - cur.len + cur.tiles - 1) - cta + 1);
       }
       const int last_page = cur.s.pos >> p.page_shift;
+      Piece nxt{};
+      int ahead = -1, nxt_base = 0, nxt_entry = -1;
       for (int i = 0; i < cur.len; ++i) {
         const int key0 = (cur.s.first() + cur.at + i) * kTile;
         const int page0 = key0 >> p.page_shift, line = key0 & ((1 << p.page_shift) - 1) & -box_lines;
@@ -323,45 +343,58 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
           bad = true;
           page = p.n_pages;
         }
-        if (!mbar_wait_warp(&empty[stage], phase ^ 1u, p.status, kStatusTimeoutAttention, abort_flag)) {
+        int id[kTile / 8];
+#pragma unroll
+        for (int b = 0; b < kTile / 8; ++b) id[b] = __shfl_sync(0xffffffffu, page, (page0 - base + b) & 31);
+        if (!wait_warp(&empty[stage], phase ^ 1u, p.status, abort_flag)) {
           ok = false;
           break;
         }
         uint8_t* buf = stages + stage * C::kStageBytes;
         if (lane == 0) {
-          TileInfo& t = info[stage];
-          t.query = cur.query;
-          t.group = cur.group;
-          t.key0 = key0;
-          t.lo = cur.s.lo;
-          t.hi = cur.s.hi;
-          t.pos = cur.s.pos;
-          t.out = out;
-          t.flags = (i == 0 ? 1 : 0) | (i == cur.len - 1 ? 2 : 0);
-          mbar_arrive_expect_tx(&full[stage], 2 * C::kKvBytes + (i == 0 ? live_rows * D * 2 : 0));
-          if (i == 0)
+          if (is_k) {
+            TileInfo& t = info[stage];
+            t.query = cur.query;
+            t.group = cur.group;
+            t.key0 = key0;
+            t.lo = cur.s.lo;
+            t.hi = cur.s.hi;
+            t.pos = cur.s.pos;
+            t.out = out;
+            t.flags = (i == 0 ? 1 : 0) | (i == cur.len - 1 ? 2 : 0);
+          }
+          const bool with_q = is_k && i == 0;
+          mbar_arrive_expect_tx(&full[stage], C::kKvBytes + (with_q ? live_rows * D * 2 : 0));
+          uint8_t* dst = buf + (is_k ? 0 : C::kKvBytes);
+#pragma unroll
+          for (int b = 0; b < kTile / 8; ++b)
+            if (b < boxes) tma_load_page(dst + b * box_lines * D * 2, map, &full[stage], line, kv_head, id[b]);
+          if (with_q)
             bulk_load(buf + 2 * C::kKvBytes,
                       static_cast<const T*>(p.q) + (static_cast<long long>(cur.query) * p.Hq + kv_head * p.G + row0) * D,
                       live_rows * D * 2, &full[stage]);
         }
-        for (int b = 0; b < boxes; ++b) {
-          const int id = __shfl_sync(0xffffffffu, page, page0 - base + b);
-          if (lane == 0) {
-            tma_load_page(buf + b * box_lines * D * 2, &tk, &full[stage], line, kv_head, id);
-            tma_load_page(buf + C::kKvBytes + b * box_lines * D * 2, &tv, &full[stage], line, kv_head, id);
-          }
-        }
+        __syncwarp();
         ++issued;
         if (++stage == C::kStages) {
           stage = 0;
           phase ^= 1u;
+        }
+        if (i == 0) {  // look ahead once the first copies are out
+          ahead = entries(cur.s, base + 32);
+          bad |= p.positions[cur.query] != cur.s.pos;
+          nxt = next_piece();
+          if (nxt.len > 0) {
+            nxt_base = first_page(nxt);
+            nxt_entry = entries(nxt.s, nxt_base);
+          }
         }
       }
       cur = nxt;
       base = nxt_base;
       entry = nxt_entry;
     }
-    if (lane == 0) p.joins[cta] = join;
+    if (is_k && lane == 0) p.joins[cta] = join;
     if (__any_sync(0xffffffffu, bad) && lane == 0) record_status(p.status, kStatusBadArgument);
     if (!ok) {  // given up: no copy may land after the CTA is gone
       for (int i = 0; i < C::kStages && i < issued; ++i) {
@@ -396,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
   int stage = 0;
   uint32_t phase = 0, merge_phase = 0;
   for (int it = 0; it < count; ++it) {
-    if (!mbar_wait_warp(&full[stage], phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
+    if (!wait_warp(&full[stage], phase, p.status, abort_flag)) return;
     const TileInfo t = info[stage];
     const uint32_t k_addr = base_addr + stage * C::kStageBytes, v_addr = k_addr + C::kKvBytes;
     if (t.flags & 1) {
@@ -550,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
         if (mr >= live_rows) break;
         __syncwarp();
         if (lane == 0) mbar_arrive(&merge);  // done with this stage, and with what was merged before
-        if (!mbar_wait_warp(&merge, merge_phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
+        if (!wait_warp(&merge, merge_phase, p.status, abort_flag)) return;
         merge_phase ^= 1u;
 #pragma unroll
         for (int nb = mr / 8; nb < (mr + C::kMergeRows) / 8; ++nb)
@@ -569,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
           }
         __syncwarp();
         if (lane == 0) mbar_arrive(&merge);
-        if (!mbar_wait_warp(&merge, merge_phase, p.status, kStatusTimeoutAttention, abort_flag)) return;
+        if (!wait_warp(&merge, merge_phase, p.status, abort_flag)) return;
         merge_phase ^= 1u;
         const int rows_here = min(C::kMergeRows, live_rows - mr);
         for (int i = tid; i < rows_here * (D / 4); i += 32 * kWarps) {

@@ -183,80 +183,111 @@ struct AppendParams {
   float eps;
 };
 
-// D / 8 lanes own one head row: lane l holds elements 8l .. 8l+7 (16-byte accesses), its rotation
-// partner (j +- D / 2) is lane l ^ (D / 16). Norm and rotation in fp32, rounded once on the store.
+// D / 16 lanes own a head row: lane l holds elements 8l .. 8l+7 and, 16 bytes each as well, their rotation
+// partners D / 2 further on, so the rotation needs no exchange and 8 cosines and sines serve 16 elements. A
+// group of lanes takes kAppendRows consecutive rows (heads) of one token: all their loads are issued before the
+// first reduction (128 bytes per thread in flight), and position, slot, cosines and sines are read once for
+// them. Norm and rotation in fp32, rounded once on the store. Bound by HBM: every row is read and written once.
+constexpr int kAppendRows = 4;
+constexpr int kAppendThreads = 128;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
-  constexpr int L = D / 8;
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) {
+  constexpr int L = D / 16;
   const int hl = threadIdx.x % L;
   const int H = p.Hq + 2 * p.Hkv;
-  const long long item = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / L;
-  const bool live = item < static_cast<long long>(p.N) * H;
-  const int m = live ? static_cast<int>(item / H) : 0;
-  const int hh = live ? static_cast<int>(item - static_cast<long long>(m) * H) : 0;
-  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.qkv) + m * p.qkv_stride + hh * D + hl * 8);
+  const int units = (H + kAppendRows - 1) / kAppendRows;  // per token
+  const unsigned unit = blockIdx.x * (kAppendThreads / L) + threadIdx.x / L;
+  // lanes past the end repeat the last token's first rows and store nothing: every lane takes part in the shuffles
+  const bool live = unit < static_cast<unsigned>(p.N) * units;
+  const int m = live ? unit / units : p.N - 1;
+  const int r0 = live ? (unit - m * units) * kAppendRows : 0;
+  const T* src = static_cast<const T*>(p.qkv) + m * p.qkv_stride + hl * 8;
+  uint4 raw[kAppendRows][2];
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    const T* row = src + min(r0 + u, H - 1) * D;
+    raw[u][0] = *reinterpret_cast<const uint4*>(row);
+    raw[u][1] = *reinterpret_cast<const uint4*>(row + D / 2);
+  }
   const int pos = p.positions[m], slot = p.slots[m];
-  const bool is_q = hh < p.Hq, is_v = hh >= p.Hq + p.Hkv;
   const bool known = pos >= 0 && (p.cos_t == nullptr || pos < p.table_len);
-  const bool stored = known && slot >= 0 && (slot >> p.page_shift) < p.n_pages;
-  if (live && hl == 0 && ((pos >= 0 && !known) || (slot >= 0 && (slot >> p.page_shift) >= p.n_pages)))
-    record_status(p.status, kStatusBadArgument);
-  uint4 out = raw;
-  if (!is_v) {
-    float x[8], w[8];
-    unpack8<T>(raw, x);
-    load8((is_q ? p.qs : p.ks) + hl * 8, w);
+  const bool in_pool = slot >= 0 && (slot >> p.page_shift) < p.n_pages;
+  if (live && hl == 0 && ((pos >= 0 && !known) || (slot >= 0 && !in_pool))) record_status(p.status, kStatusBadArgument);
+  float c[8], sn[8];
+  if (p.cos_t != nullptr) {
+    const long long at = static_cast<long long>(known ? pos : 0) * (D / 2) + hl * 8;
+    load8(p.cos_t + at, c);
+    load8(p.sin_t + at, sn);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
+  }
+  const long long page = slot >> p.page_shift, line = slot & ((1 << p.page_shift) - 1);
+  T* const kp = static_cast<T*>(p.kp) + page * p.kp_page + line * p.kp_line + hl * 8;
+  T* const vp = static_cast<T*>(p.vp) + page * p.vp_page + line * p.vp_line + hl * 8;
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    const int r = r0 + u;
+    const bool is_q = r < p.Hq, is_v = r >= p.Hq + p.Hkv;
+    float a[8], b[8];
+    unpack8<T>(raw[u][0], a);
+    unpack8<T>(raw[u][1], b);
     float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-    // the butterfly stays inside the row's L lanes; rows of one warp may differ in kind (q, k, v),
-    // so only the row's own lanes take part
-    const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
+    for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
 #pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(mask, ss, d);
-    const float r = rsqrtf(ss / D + p.eps);
+    for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    const float norm = rsqrtf(ss / D + p.eps);
+    const float* scale = (is_q ? p.qs : p.ks) + hl * 8;
+    float wa[8], wb[8];
+    load8(scale, wa);
+    load8(scale + D / 2, wb);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= r * (1.f + w[e]);
-    if (p.cos_t != nullptr) {
-      const long long at = static_cast<long long>(known ? pos : 0) * (D / 2) + (hl % (L / 2)) * 8;
-      float c[8], s[8];
-      load8(p.cos_t + at, c);
-      load8(p.sin_t + at, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float partner = __shfl_xor_sync(mask, x[e], L / 2);
-        x[e] = hl < L / 2 ? x[e] * c[e] - partner * s[e] : partner * s[e] + x[e] * c[e];
-      }
+    for (int e = 0; e < 8; ++e) {
+      const float x = a[e] * norm * (1.f + wa[e]), y = b[e] * norm * (1.f + wb[e]);
+      a[e] = x * c[e] - y * sn[e];
+      b[e] = x * sn[e] + y * c[e];
     }
-    out = pack8<T>(x);
+    uint4 lo = is_v ? raw[u][0] : pack8<T>(a), hi = is_v ? raw[u][1] : pack8<T>(b);
+    if (!known) lo = hi = make_uint4(0, 0, 0, 0);
+    if (!live || r >= H) continue;
+    if (is_q) {
+      T* dst = static_cast<T*>(p.q) + (static_cast<long long>(m) * p.Hq + r) * D + hl * 8;
+      *reinterpret_cast<uint4*>(dst) = lo;
+      *reinterpret_cast<uint4*>(dst + D / 2) = hi;
+      continue;
+    }
+    const int hk = is_v ? r - p.Hq - p.Hkv : r - p.Hq;
+    T* dense = static_cast<T*>(is_v ? p.v : p.k);
+    if (dense != nullptr) {
+      dense += (static_cast<long long>(m) * p.Hkv + hk) * D + hl * 8;
+      *reinterpret_cast<uint4*>(dense) = lo;
+      *reinterpret_cast<uint4*>(dense + D / 2) = hi;
+    }
+    if (known && in_pool) {
+      T* dst = is_v ? vp + hk * p.vp_head : kp + hk * p.kp_head;
+      *reinterpret_cast<uint4*>(dst) = lo;
+      *reinterpret_cast<uint4*>(dst + D / 2) = hi;
+    }
   }
-  if (!known) out = make_uint4(0, 0, 0, 0);
-  if (!live) return;
-  if (is_q) {
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.q) + (static_cast<long long>(m) * p.Hq + hh) * D + hl * 8) = out;
-    return;
-  }
-  const int hk = is_v ? hh - p.Hq - p.Hkv : hh - p.Hq;
-  T* dense = static_cast<T*>(is_v ? p.v : p.k);
-  if (dense != nullptr)
-    *reinterpret_cast<uint4*>(dense + (static_cast<long long>(m) * p.Hkv + hk) * D + hl * 8) = out;
-  if (!stored) return;
-  const long long page = slot >> p.page_shift, line = slot & ((1 << p.page_shift) - 1);
-  T* dst = is_v ? static_cast<T*>(p.vp) + page * p.vp_page + hk * p.vp_head + line * p.vp_line
-                : static_cast<T*>(p.kp) + page * p.kp_page + hk * p.kp_head + line * p.kp_line;
-  *reinterpret_cast<uint4*>(dst + hl * 8) = out;
+}
+
+template <typename T, int D>
+void launch_append(const AppendParams& p, cudaStream_t st) {
+  const int64_t units = static_cast<int64_t>(p.N) * ((p.Hq + 2 * p.Hkv + kAppendRows - 1) / kAppendRows);
+  constexpr int kPerBlock = kAppendThreads / (D / 16);
+  append_kernel<T, D><<<static_cast<unsigned>((units + kPerBlock - 1) / kPerBlock), kAppendThreads, 0, st>>>(p);
 }
 
 template <typename T>
-void launch_append(const AppendParams& p, int D, cudaStream_t st) {
-  const long long threads = static_cast<long long>(p.N) * (p.Hq + 2 * p.Hkv) * (D / 8);
-  const unsigned grid = static_cast<unsigned>((threads + 255) / 256);
+void launch_append(const AppendParams& p, int64_t D, cudaStream_t st) {
   if (D == 64) {
-    append_kernel<T, 64><<<grid, 256, 0, st>>>(p);
+    launch_append<T, 64>(p, st);
   } else if (D == 128) {
-    append_kernel<T, 128><<<grid, 256, 0, st>>>(p);
+    launch_append<T, 128>(p, st);
   } else {
-    append_kernel<T, 256><<<grid, 256, 0, st>>>(p);
+    launch_append<T, 256>(p, st);
   }
 }
 
@@ -369,7 +400,7 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
     out.push_back(at::empty({N, n_kv, D}, opts));
   }
   if (N == 0) return out;
-  MINT_CHECK(N * (n_q + 2 * n_kv) * (D / 8) < (1ll << 38), "qk_norm_rope_paged: too many tokens for one call");
+  MINT_CHECK(N * (n_q + 2 * n_kv) < (1ll << 31), "qk_norm_rope_paged: too many rows for one call");
   c10::cuda::CUDAGuard guard(qkv.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   p.qkv = qkv.data_ptr();
@@ -397,9 +428,9 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
   p.n_pages = static_cast<int>(kp.size(0));
   p.eps = static_cast<float>(eps);
   if (dt == at::kBFloat16) {
-    paged::launch_append<__nv_bfloat16>(p, static_cast<int>(D), stream);
+    paged::launch_append<__nv_bfloat16>(p, D, stream);
   } else {
-    paged::launch_append<__half>(p, static_cast<int>(D), stream);
+    paged::launch_append<__half>(p, D, stream);
   }
   MINT_CUDA_CHECK(cudaGetLastError());
   count_launch();
