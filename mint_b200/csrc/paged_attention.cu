@@ -29,6 +29,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "paged.cuh"
@@ -718,16 +719,20 @@ void launch_attend(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, c
   using C = Config<D, NB>;
   const int device = q.device().index();
   const auto kernel = attend_kernel<T, D, NB, TWIN>;
-  check_smem_optin(C::kSmem, device, "paged_attention");
-  MINT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised for this kernel
+  if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
+    check_smem_optin(C::kSmem, device, "paged_attention");
+    MINT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    ready.fetch_or(1ull << device, std::memory_order_relaxed);
+  }
   const int grid = num_sms(device) * (C::kTwo ? 2 : 1);
   p.groups = (p.G + C::kRows - 1) / C::kRows;
   p.part_rows = p.groups > 1 ? C::kRows : p.G;
   const int64_t slots = 2ll * grid * p.part_rows;
-  auto ws = at::empty({slots * (D + 2) + 4 * grid}, q.options().dtype(at::kFloat));
-  p.part_o = ws.data_ptr<float>();
+  auto ws = empty_cuda({may_split ? slots * (D + 2) + 4 * grid : 4 * grid}, at::kFloat, q.device());
+  p.joins = reinterpret_cast<int4*>(ws.data_ptr<float>());
+  p.part_o = ws.data_ptr<float>() + 4 * grid;
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * D);
-  p.joins = reinterpret_cast<int4*>(p.part_o + slots * (D + 2));
   // tile numbers are ints: so many queries that they might not fit go in several launches
   const int64_t per_query = tiles_bound * p.Hkv * p.groups;
   MINT_CHECK(per_query <= INT_MAX, "paged_attention: a query may have too many tiles");
@@ -794,6 +799,7 @@ void dispatch_dim(const AttnParams& p, int64_t D, Args&&... args) {
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& tables,
                            const at::Tensor& positions, const c10::optional<at::Tensor>& rows, int64_t window,
                            const c10::optional<at::Tensor>& slopes, double scale) {
+  paged::check_inference("paged_attention", {&q, &kp, &vp});
   check_contig(q, "q");
   check_cuda(tables, "block_tables");
   check_contig(positions, "positions");
@@ -827,7 +833,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::
                "alibi_slopes are fp32, one per query head");
     p.slopes = slopes->data_ptr<float>();
   }
-  auto o = at::empty_like(q);
+  auto o = paged::empty_cuda(q.sizes(), dt, q.device());
   if (N == 0) return o;
   const int shift = paged::shift_of(kp.size(2));
   MINT_CHECK(N < (1 << 24) && Hq < (1 << 16) && tables.size(0) < (1ll << 31) && tables.size(1) <= (INT_MAX >> shift),

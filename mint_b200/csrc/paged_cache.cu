@@ -184,100 +184,154 @@ struct AppendParams {
 };
 
 // D / 16 lanes own a head row: lane l holds elements 8l .. 8l+7 and, 16 bytes each as well, their rotation
-// partners D / 2 further on, so the rotation needs no exchange and 8 cosines and sines serve 16 elements. A
-// group of lanes takes kAppendRows consecutive rows (heads) of one token: all their loads are issued before the
-// first reduction (128 bytes per thread in flight), and position, slot, cosines and sines are read once for
-// them. Norm and rotation in fp32, rounded once on the store. Bound by HBM: every row is read and written once.
-constexpr int kAppendRows = 4;
-constexpr int kAppendThreads = 128;
-
+// partners D / 2 further on, so the rotation needs no exchange and 8 cosines and sines serve 16 elements. Norm
+// and rotation in fp32, rounded once on the store.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) {
-  constexpr int L = D / 16;
-  const int hl = threadIdx.x % L;
-  const int H = p.Hq + 2 * p.Hkv;
-  const int units = (H + kAppendRows - 1) / kAppendRows;  // per token
-  const unsigned unit = blockIdx.x * (kAppendThreads / L) + threadIdx.x / L;
-  // lanes past the end repeat the last token's first rows and store nothing: every lane takes part in the shuffles
-  const bool live = unit < static_cast<unsigned>(p.N) * units;
-  const int m = live ? unit / units : p.N - 1;
-  const int r0 = live ? (unit - m * units) * kAppendRows : 0;
-  const T* src = static_cast<const T*>(p.qkv) + m * p.qkv_stride + hl * 8;
-  uint4 raw[kAppendRows][2];
-#pragma unroll
-  for (int u = 0; u < kAppendRows; ++u) {
-    const T* row = src + min(r0 + u, H - 1) * D;
-    raw[u][0] = *reinterpret_cast<const uint4*>(row);
-    raw[u][1] = *reinterpret_cast<const uint4*>(row + D / 2);
+struct HeadRow {
+  static constexpr int L = D / 16;
+  uint4 lo, hi;
+
+  __device__ __forceinline__ void load(const T* row) {
+    lo = *reinterpret_cast<const uint4*>(row);
+    hi = *reinterpret_cast<const uint4*>(row + D / 2);
   }
-  const int pos = p.positions[m], slot = p.slots[m];
-  const bool known = pos >= 0 && (p.cos_t == nullptr || pos < p.table_len);
+  __device__ __forceinline__ void store(T* row) const {
+    *reinterpret_cast<uint4*>(row) = lo;
+    *reinterpret_cast<uint4*>(row + D / 2) = hi;
+  }
+  // all lanes of the warp call it (the sum runs over the row's L lanes); w = 1 + scale of the two halves
+  __device__ __forceinline__ void norm_rotate(const float2 (&w)[2][4], const float2 (&c)[4], const float2 (&sn)[4],
+                                              float eps) {
+    float2 a[4], b[4], sum = make_float2(0.f, 0.f), sum2 = make_float2(0.f, 0.f);
+    unpack8<T>(lo, a);
+    unpack8<T>(hi, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum = ffma2(a[e], a[e], sum);
+      sum2 = ffma2(b[e], b[e], sum2);
+    }
+    sum = fadd2(sum, sum2);
+    float ss = sum.x + sum.y;
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    const float norm = rsqrtf(ss * (1.f / D) + eps);
+    const float2 n2 = make_float2(norm, norm), minus = make_float2(-norm, -norm);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = fmul2(a[e], w[0][e]), y = fmul2(b[e], w[1][e]);
+      a[e] = ffma2(fmul2(x, c[e]), n2, fmul2(fmul2(y, sn[e]), minus));
+      b[e] = fmul2(ffma2(x, sn[e], fmul2(y, c[e])), n2);
+    }
+    lo = pack8<T>(a);
+    hi = pack8<T>(b);
+  }
+};
+
+struct Place {  // where a token goes
+  bool known, stored;
+  long long page, line;
+};
+__device__ __forceinline__ Place place_of(const AppendParams& p, int pos, int slot, bool report) {
+  Place t;
+  t.known = pos >= 0 && (p.cos_t == nullptr || pos < p.table_len);
   const bool in_pool = slot >= 0 && (slot >> p.page_shift) < p.n_pages;
-  if (live && hl == 0 && ((pos >= 0 && !known) || (slot >= 0 && !in_pool))) record_status(p.status, kStatusBadArgument);
-  float c[8], sn[8];
+  t.stored = t.known && in_pool;
+  t.page = slot >> p.page_shift;
+  t.line = slot & ((1 << p.page_shift) - 1);
+  if (report && ((pos >= 0 && !t.known) || (slot >= 0 && !in_pool))) record_status(p.status, kStatusBadArgument);
+  return t;
+}
+
+// 1 + scale of a q or k row's two halves
+template <int D>
+__device__ __forceinline__ void load_scale(const AppendParams& p, bool is_q, int hl, float2 (&w)[2][4]) {
+  const float* scale = (is_q ? p.qs : p.ks) + hl * 8;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    load8(scale + h * (D / 2), w[h]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[h][e] = make_float2(w[h][e].x + 1.f, w[h][e].y + 1.f);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_turn(const AppendParams& p, int pos, int hl, float2 (&c)[4], float2 (&sn)[4]) {
   if (p.cos_t != nullptr) {
-    const long long at = static_cast<long long>(known ? pos : 0) * (D / 2) + hl * 8;
+    const long long at = static_cast<long long>(pos) * (D / 2) + hl * 8;
     load8(p.cos_t + at, c);
     load8(p.sin_t + at, sn);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = 1.f, sn[e] = 0.f;
-  }
-  const long long page = slot >> p.page_shift, line = slot & ((1 << p.page_shift) - 1);
-  T* const kp = static_cast<T*>(p.kp) + page * p.kp_page + line * p.kp_line + hl * 8;
-  T* const vp = static_cast<T*>(p.vp) + page * p.vp_page + line * p.vp_line + hl * 8;
-#pragma unroll
-  for (int u = 0; u < kAppendRows; ++u) {
-    const int r = r0 + u;
-    const bool is_q = r < p.Hq, is_v = r >= p.Hq + p.Hkv;
-    float a[8], b[8];
-    unpack8<T>(raw[u][0], a);
-    unpack8<T>(raw[u][1], b);
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
-#pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    const float norm = rsqrtf(ss / D + p.eps);
-    const float* scale = (is_q ? p.qs : p.ks) + hl * 8;
-    float wa[8], wb[8];
-    load8(scale, wa);
-    load8(scale + D / 2, wb);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = a[e] * norm * (1.f + wa[e]), y = b[e] * norm * (1.f + wb[e]);
-      a[e] = x * c[e] - y * sn[e];
-      b[e] = x * sn[e] + y * c[e];
-    }
-    uint4 lo = is_v ? raw[u][0] : pack8<T>(a), hi = is_v ? raw[u][1] : pack8<T>(b);
-    if (!known) lo = hi = make_uint4(0, 0, 0, 0);
-    if (!live || r >= H) continue;
-    if (is_q) {
-      T* dst = static_cast<T*>(p.q) + (static_cast<long long>(m) * p.Hq + r) * D + hl * 8;
-      *reinterpret_cast<uint4*>(dst) = lo;
-      *reinterpret_cast<uint4*>(dst + D / 2) = hi;
-      continue;
-    }
-    const int hk = is_v ? r - p.Hq - p.Hkv : r - p.Hq;
-    T* dense = static_cast<T*>(is_v ? p.v : p.k);
-    if (dense != nullptr) {
-      dense += (static_cast<long long>(m) * p.Hkv + hk) * D + hl * 8;
-      *reinterpret_cast<uint4*>(dense) = lo;
-      *reinterpret_cast<uint4*>(dense + D / 2) = hi;
-    }
-    if (known && in_pool) {
-      T* dst = is_v ? vp + hk * p.vp_head : kp + hk * p.kp_head;
-      *reinterpret_cast<uint4*>(dst) = lo;
-      *reinterpret_cast<uint4*>(dst + D / 2) = hi;
-    }
+    for (int e = 0; e < 4; ++e) c[e] = make_float2(1.f, 1.f), sn[e] = make_float2(0.f, 0.f);
   }
 }
 
 template <typename T, int D>
+__device__ __forceinline__ void write_row(const AppendParams& p, const Place& t, HeadRow<T, D>& x, int m, int r, int hl) {
+  if (!t.known) x.lo = x.hi = make_uint4(0, 0, 0, 0);
+  if (r < p.Hq) {
+    x.store(static_cast<T*>(p.q) + (static_cast<long long>(m) * p.Hq + r) * D + hl * 8);
+    return;
+  }
+  const bool is_v = r >= p.Hq + p.Hkv;
+  const int hk = is_v ? r - p.Hq - p.Hkv : r - p.Hq;
+  T* dense = static_cast<T*>(is_v ? p.v : p.k);
+  if (dense != nullptr) x.store(dense + (static_cast<long long>(m) * p.Hkv + hk) * D + hl * 8);
+  if (t.stored)
+    x.store((is_v ? static_cast<T*>(p.vp) + t.page * p.vp_page + hk * p.vp_head + t.line * p.vp_line
+                  : static_cast<T*>(p.kp) + t.page * p.kp_page + hk * p.kp_head + t.line * p.kp_line) + hl * 8);
+}
+
+// A group of lanes takes ROWS consecutive rows (heads) of one token: all their loads are issued before the
+// first reduction, and position, slot, cosines and sines are read once for them.
+constexpr int kAppendThreads = 64;
+constexpr int64_t kTwoRowsBytes = 3 << 20;
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kAppendThreads, ROWS == 1 ? 1 : 16) append_kernel(AppendParams p) {
+  using Row = HeadRow<T, D>;
+  const int hl = threadIdx.x % Row::L;
+  const int H = p.Hq + 2 * p.Hkv;
+  const int units = (H + ROWS - 1) / ROWS;  // per token
+  const unsigned unit = blockIdx.x * (kAppendThreads / Row::L) + threadIdx.x / Row::L;
+  // lanes past the end repeat the last token's first rows and store nothing: every lane takes part in the sums
+  const bool live = unit < static_cast<unsigned>(p.N) * units;
+  const int m = live ? unit / units : p.N - 1;
+  const int r0 = live ? (unit - m * units) * ROWS : 0;
+  const T* src = static_cast<const T*>(p.qkv) + m * p.qkv_stride + hl * 8;
+  Row x[ROWS];
+#pragma unroll
+  for (int u = 0; u < ROWS; ++u) x[u].load(src + min(r0 + u, H - 1) * D);
+  const int pos = p.positions[m], slot = p.slots[m];
+  float2 w[2][4], c[4], sn[4];
+  if (ROWS == 1) load_scale<D>(p, r0 < p.Hq, hl, w);
+  const Place t = place_of(p, pos, slot, live && r0 == 0 && hl == 0);
+  load_turn<D>(p, t.known ? pos : 0, hl, c, sn);
+#pragma unroll
+  for (int u = 0; u < ROWS; ++u) {
+    const int r = r0 + u;
+    const Row raw = x[u];
+    if (ROWS > 1) load_scale<D>(p, r < p.Hq, hl, w);
+    x[u].norm_rotate(w, c, sn, p.eps);
+    if (r >= p.Hq + p.Hkv) x[u] = raw;
+    if (live && r < H) write_row<T, D>(p, t, x[u], m, r, hl);
+  }
+}
+
+template <typename T, int D, int ROWS>
 void launch_append(const AppendParams& p, cudaStream_t st) {
-  const int64_t units = static_cast<int64_t>(p.N) * ((p.Hq + 2 * p.Hkv + kAppendRows - 1) / kAppendRows);
+  const int64_t units = static_cast<int64_t>(p.N) * ((p.Hq + 2 * p.Hkv + ROWS - 1) / ROWS);
   constexpr int kPerBlock = kAppendThreads / (D / 16);
-  append_kernel<T, D><<<static_cast<unsigned>((units + kPerBlock - 1) / kPerBlock), kAppendThreads, 0, st>>>(p);
+  append_kernel<T, D, ROWS><<<static_cast<unsigned>((units + kPerBlock - 1) / kPerBlock), kAppendThreads, 0, st>>>(p);
+}
+
+template <typename T, int D>
+void launch_append(const AppendParams& p, cudaStream_t st) {
+  if (static_cast<int64_t>(p.N) * (p.Hq + 2 * p.Hkv) * D * 2 < kTwoRowsBytes) {
+    launch_append<T, D, 1>(p, st);
+  } else {
+    launch_append<T, D, 2>(p, st);
+  }
 }
 
 template <typename T>
@@ -314,10 +368,12 @@ std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fres
   MINT_CHECK(free_head.numel() == 1, "free_head has one element");
   MINT_CHECK(n_tokens >= 0 && n_tokens <= paged::kLenCap && tables.size(1) < (1ll << 31) && free_pages.numel() < (1ll << 31),
              "paged_plan sizes");
-  auto opts = seq.options();
-  auto tok = at::empty({3, n_tokens}, opts);
-  auto req = at::empty({2, B}, opts);
-  auto head = at::empty({1}, opts);
+  // one allocation for the outputs; each starts on a 16-byte boundary
+  auto round4 = [](int64_t n) { return (n + 3) / 4 * 4; };
+  const int64_t nt = round4(n_tokens), nb = round4(B);
+  auto out = paged::empty_cuda({3 * nt + 2 * nb + 4}, at::kInt, seq.device());
+  std::vector<at::Tensor> views{paged::flat_view(out, 0, n_tokens),      paged::flat_view(out, nt, n_tokens), paged::flat_view(out, 2 * nt, n_tokens),
+                                paged::flat_view(out, 3 * nt, B),        paged::flat_view(out, 3 * nt + nb, B), paged::flat_view(out, 3 * nt + 2 * nb, 1)};
   c10::cuda::CUDAGuard guard(seq.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   paged::PlanParams p{};
@@ -326,12 +382,12 @@ std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fres
   p.tables = tables.data_ptr<int>();
   p.free_pages = free_pages.data_ptr<int>();
   p.free_head = free_head.data_ptr<int>();
-  p.positions = tok.data_ptr<int>();
-  p.slots = p.positions + n_tokens;
-  p.rows = p.slots + n_tokens;
-  p.ends = req.data_ptr<int>();
-  p.seq_out = p.ends + B;
-  p.head_out = head.data_ptr<int>();
+  p.positions = out.data_ptr<int>();
+  p.slots = p.positions + nt;
+  p.rows = p.slots + nt;
+  p.ends = p.rows + nt;
+  p.seq_out = p.ends + nb;
+  p.head_out = p.seq_out + nb;
   p.status = status_ptr(seq.device().index());
   p.tstride = tables.stride(0);
   p.B = static_cast<int>(B);
@@ -349,7 +405,7 @@ std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fres
   paged::plan_kernel<<<grid, paged::kPlanThreads, smem, stream>>>(p);
   MINT_CUDA_CHECK(cudaGetLastError());
   count_launch();
-  return {tok.select(0, 0), tok.select(0, 1), tok.select(0, 2), req.select(0, 0), req.select(0, 1), head};
+  return views;
 }
 
 // q [N, Hq, D] normed and rotated; k (normed, rotated) and v stored into the pools' slots. With `dense`
@@ -360,6 +416,7 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
                                            const c10::optional<at::Tensor>& sin_t, const at::Tensor& positions,
                                            const at::Tensor& slots, at::Tensor& kp, at::Tensor& vp, double eps,
                                            bool dense) {
+  paged::check_inference("qk_norm_rope_paged", {&qkv, &qs, &ks, &kp, &vp});
   check_cuda(qkv, "qkv");
   check_contig(positions, "positions");
   check_contig(slots, "slots");
@@ -368,7 +425,8 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
   const auto dt = qkv.scalar_type();
   MINT_CHECK((dt == at::kBFloat16 || dt == at::kHalf) && (D == 64 || D == 128 || D == 256),
              "qk_norm_rope_paged takes bf16 or fp16 heads of 64, 128 or 256");
-  MINT_CHECK(n_q >= 1 && n_kv >= 1 && qkv.dim() == 2 && qkv.size(1) == (n_q + 2 * n_kv) * D, "qkv width mismatch");
+  MINT_CHECK(n_q >= 1 && n_kv >= 1 && qkv.dim() == 2 && qkv.size(1) == (n_q + 2 * n_kv) * D, "qkv must be [N, ",
+             (n_q + 2 * n_kv) * D, "]");
   MINT_CHECK(qkv.stride(1) == 1 && qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
              "qkv rows must be contiguous and 16-byte aligned");
   const int64_t N = qkv.size(0);
@@ -380,6 +438,8 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
   paged::check_pool(kp, "k_pages", dt, n_kv, D);
   paged::check_pool(vp, "v_pages", dt, n_kv, D);
   MINT_CHECK(kp.sizes() == vp.sizes(), "k_pages and v_pages have different shapes");
+  for (const at::Tensor* t : {&positions, &slots, &qs, &ks, static_cast<const at::Tensor*>(&kp), static_cast<const at::Tensor*>(&vp)})
+    MINT_CHECK(t->device() == qkv.device(), "qk_norm_rope_paged takes tensors on one device");
   paged::AppendParams p{};
   if (cos_t.has_value()) {
     MINT_CHECK(sin_t.has_value(), "rotation needs both cos and sin");
@@ -388,16 +448,16 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
     MINT_CHECK(cos_t->scalar_type() == at::kFloat && sin_t->scalar_type() == at::kFloat && cos_t->dim() == 2 &&
                    cos_t->size(1) == D / 2 && cos_t->sizes() == sin_t->sizes(),
                "cos / sin are fp32 [positions, head_dim / 2]");
+    MINT_CHECK(cos_t->device() == qkv.device() && sin_t->device() == qkv.device(), "qk_norm_rope_paged takes tensors on one device");
     p.cos_t = cos_t->data_ptr<float>();
     p.sin_t = sin_t->data_ptr<float>();
     p.table_len = static_cast<int>(std::min<int64_t>(cos_t->size(0), INT32_MAX));
   }
-  auto opts = qkv.options();
-  auto q = at::empty({N, n_q, D}, opts);
+  auto q = paged::empty_cuda({N, n_q, D}, dt, qkv.device());
   std::vector<at::Tensor> out{q};
   if (dense) {
-    out.push_back(at::empty({N, n_kv, D}, opts));
-    out.push_back(at::empty({N, n_kv, D}, opts));
+    out.push_back(paged::empty_cuda({N, n_kv, D}, dt, qkv.device()));
+    out.push_back(paged::empty_cuda({N, n_kv, D}, dt, qkv.device()));
   }
   if (N == 0) return out;
   MINT_CHECK(N * (n_q + 2 * n_kv) < (1ll << 31), "qk_norm_rope_paged: too many rows for one call");

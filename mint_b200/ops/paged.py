@@ -31,6 +31,7 @@ from mint_b200.ops.norm import _rms_ref
 from mint_b200.ops.rope import _rotate_ref
 
 _HEAD_DIMS = (64, 128, 256)
+_KERNEL_DTYPES = (torch.bfloat16, torch.float16)
 
 
 class PagedPlan(NamedTuple):
@@ -103,10 +104,10 @@ def paged_plan(
     CUDA: one kernel, no host synchronization. What cannot be placed (no page left, a request longer than
     its table row, more new tokens than ``n_tokens``) gets slot -1 and "bad kernel argument" in the
     device status word; CPU tensors raise ValueError."""
-    check_page_size(page_size)
     if _ext.use_cuda_kernels(seq_lens):
         return PagedPlan(*_ext.require().paged_plan(seq_lens, new_lens, block_tables, free_pages, free_head,
                                                     page_size, n_tokens))
+    check_page_size(page_size)
     return _plan_ref(seq_lens, new_lens, block_tables, free_pages, free_head, page_size, n_tokens)
 
 
@@ -161,18 +162,20 @@ def qk_norm_rope_paged(
     rotation. Norm and rotation are computed in fp32 and rounded once. A token with slot -1 is not
     stored; one whose position or slot is out of range is not stored either and is reported in the
     device status word (CPU tensors raise ValueError)."""
+    if _ext.use_cuda_kernels(qkv):
+        if qkv.dtype in _KERNEL_DTYPES and head_dim in _HEAD_DIMS:
+            if q_scale.dtype != torch.float32 or k_scale.dtype != torch.float32:
+                q_scale, k_scale = q_scale.float(), k_scale.float()
+            out = _ext.require().qk_norm_rope_paged(qkv, n_q, n_kv, head_dim, q_scale, k_scale, cos, sin, positions, slots,
+                                                    k_pages, v_pages, eps, return_kv)
+            return tuple(out) if return_kv else out[0]
+        _ext.fallback("qk_norm_rope_paged", "dtype / head_dim without a kernel")
     _inference_only("qk_norm_rope_paged", qkv, q_scale, k_scale, k_pages, v_pages)
     if qkv.dim() != 2 or qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
         raise ValueError(f"qkv must be [N, {(n_q + 2 * n_kv) * head_dim}], got {tuple(qkv.shape)}")
     if k_pages.dtype != qkv.dtype or v_pages.dtype != qkv.dtype:
         raise ValueError(f"qkv is {qkv.dtype} but the pages are {k_pages.dtype} / {v_pages.dtype}")
     check_page_size(k_pages.shape[2])
-    if _ext.use_cuda_kernels(qkv):
-        if qkv.dtype in (torch.bfloat16, torch.float16) and head_dim in _HEAD_DIMS:
-            out = _ext.require().qk_norm_rope_paged(qkv, n_q, n_kv, head_dim, q_scale.float(), k_scale.float(), cos, sin,
-                                                    positions, slots, k_pages, v_pages, eps, return_kv)
-            return tuple(out) if return_kv else out[0]
-        _ext.fallback("qk_norm_rope_paged", "dtype / head_dim without a kernel")
     q, k, v = _append_ref(qkv, n_q, n_kv, head_dim, q_scale, k_scale, cos, sin, positions, slots, k_pages, v_pages, eps)
     return (q, k, v) if return_kv else q
 
@@ -221,6 +224,12 @@ def paged_attention(
     adds ``slope * (j - position)`` to the scores. Queries with position -1 (or a row out of range)
     return zeros. Whatever the pages hold outside the keys seen is ignored, NaN included. Several
     queries of one request may be passed: each is computed on its own."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if _ext.use_cuda_kernels(q):
+        if q.dtype in _KERNEL_DTYPES and q.shape[-1] in _HEAD_DIMS:
+            return _ext.require().paged_attention(q.contiguous(), k_pages, v_pages, block_tables, positions, rows,
+                                                  window_left, alibi_slopes, scale)
+        _ext.fallback("paged_attention", "dtype / head_dim without a kernel")
     _inference_only("paged_attention", q, k_pages, v_pages, alibi_slopes)
     if q.dim() != 3 or k_pages.dim() != 4 or q.shape[1] % k_pages.shape[1] or q.shape[2] != k_pages.shape[3]:
         raise ValueError(f"paged_attention: q {tuple(q.shape)} does not fit k_pages {tuple(k_pages.shape)}")
@@ -229,10 +238,4 @@ def paged_attention(
     if rows is None and block_tables.shape[0] != q.shape[0]:
         raise ValueError("paged_attention: without rows, block_tables has one row per query")
     check_page_size(k_pages.shape[2])
-    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    if _ext.use_cuda_kernels(q):
-        if q.dtype in (torch.bfloat16, torch.float16) and q.shape[2] in _HEAD_DIMS:
-            return _ext.require().paged_attention(q, k_pages, v_pages, block_tables, positions, rows, window_left,
-                                                  alibi_slopes, scale)
-        _ext.fallback("paged_attention", "dtype / head_dim without a kernel")
     return _attention_ref(q, k_pages, v_pages, block_tables, positions, rows, window_left, alibi_slopes, scale)
