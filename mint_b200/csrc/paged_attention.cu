@@ -63,7 +63,7 @@ struct Config {
   static_assert(kWarps * kMergeRows * kMergeLine * 4 <= kStageBytes, "merge buffer");
 };
 
-struct TileInfo {  // the tile in a stage, for the consumers
+struct alignas(16) TileInfo {  // the tile in a stage, for the consumers
   int query, group;  // item: query and KV head * row groups + row group
   int key0, lo, hi, pos;
   int out;    // partial slot, or -1: write the output
@@ -353,17 +353,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
         }
         uint8_t* buf = stages + stage * C::kStageBytes;
         if (lane == 0) {
-          if (is_k) {
-            TileInfo& t = info[stage];
-            t.query = cur.query;
-            t.group = cur.group;
-            t.key0 = key0;
-            t.lo = cur.s.lo;
-            t.hi = cur.s.hi;
-            t.pos = cur.s.pos;
-            t.out = out;
-            t.flags = (i == 0 ? 1 : 0) | (i == cur.len - 1 ? 2 : 0);
-          }
+          if (is_k)
+            info[stage] = TileInfo{cur.query, cur.group, key0, cur.s.lo, cur.s.hi, cur.s.pos, out,
+                                   (i == 0 ? 1 : 0) | (i == cur.len - 1 ? 2 : 0)};
           const bool with_q = is_k && i == 0;
           mbar_arrive_expect_tx(&full[stage], C::kKvBytes + (with_q ? live_rows * D * 2 : 0));
           uint8_t* dst = buf + (is_k ? 0 : C::kKvBytes);
@@ -758,7 +750,7 @@ void launch_attend(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, c
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, std::min(p.part_rows, 4));
+    cfg.gridDim = dim3(grid, std::min(p.part_rows, 16));
     cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = stream;
     cfg.attrs = &attr;
