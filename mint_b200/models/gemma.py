@@ -14,6 +14,7 @@ LM head are vocab-parallel and ``forward`` all-gathers the vocabulary shards.
 
 from __future__ import annotations
 
+from collections.abc import Sequence
 from dataclasses import dataclass, field
 from typing import Any
 
@@ -23,6 +24,7 @@ from torch import nn
 from torch.utils.checkpoint import checkpoint
 
 from mint_b200.kvcache.base import KVCache
+from mint_b200.kvcache.paged import PagedKVCache, PagedLayer
 from mint_b200.nn.base import ModelConfig, compute_dtype
 from mint_b200.nn.blocks import GQAGluBlock
 from mint_b200.nn.norm import RMSNorm
@@ -186,13 +188,18 @@ class Gemma(nn.Module):
     def forward(
         self,
         input_ids: torch.Tensor,
-        kv_caches: list[KVCache] | None = None,
+        kv_caches: list[KVCache] | list[PagedLayer] | None = None,
         start_pos: int = 0,
         doc_ids: torch.Tensor | None = None,
         attn_mask: torch.Tensor | None = None,
         unpad_logits: bool = True,
+        select: torch.Tensor | None = None,
     ) -> torch.Tensor:
+        """Logits of every token, or (``select``: token indices) of some. With a paged cache ``input_ids`` is the
+        packed row ``[1, N]`` of a :class:`~mint_b200.kvcache.paged.PagedStep` and ``kv_caches`` its layers."""
         hn = self._trunk(input_ids, kv_caches, start_pos, doc_ids, attn_mask)
+        if select is not None:
+            hn = hn[:, select]
         if type(self.output) is nn.Linear:
             logits = linear(hn, self.output.weight, compute_dtype=compute_dtype(hn))
         else:
@@ -284,32 +291,167 @@ class Gemma(nn.Module):
                 if input_ids.shape[1] > kv_caches[0].max_seq_len:
                     break
                 logits = self(input_ids[:, -1:], kv_caches=kv_caches, start_pos=input_ids.shape[1] - 1)
-            logits = logits[:, -1, :].float()
-            if temperature == 0:
-                next_token = logits.argmax(dim=-1, keepdim=True)
-            else:
-                logits = logits / temperature
-                if top_k is not None:
-                    v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
-                    logits[logits < v[:, [-1]]] = -float("inf")
-                if top_p is not None:
-                    sorted_logits, sorted_idx = torch.sort(logits, descending=True)
-                    cum = torch.cumsum(torch.softmax(sorted_logits, dim=-1), dim=-1)
-                    remove = cum > top_p
-                    remove[..., 1:] = remove[..., :-1].clone()
-                    remove[..., 0] = False
-                    logits[remove.scatter(1, sorted_idx, remove)] = -float("inf")
-                next_token = torch.multinomial(torch.softmax(logits, dim=-1), num_samples=1)
+            next_token = _sample(logits[:, -1, :].float(), temperature, top_k, top_p)
             input_ids = torch.cat([input_ids, next_token], dim=1)
             if eos_token_id is not None and (next_token == eos_token_id).all():
                 break
         return input_ids
+
+    @torch.no_grad()
+    def generate_batch(
+        self,
+        prompts: Sequence[torch.Tensor | Sequence[int]],
+        max_new_tokens: int,
+        temperature: float = 1.0,
+        top_k: int | None = None,
+        top_p: float | None = None,
+        eos_token_id: int | None = None,
+        *,
+        max_batch: int = 32,
+        page_size: int = 16,
+        cache: PagedKVCache | None = None,
+        cuda_graph: bool = True,
+    ) -> list[torch.Tensor]:
+        """Continue prompts of any lengths together; returns each prompt with its new tokens (1-D, on the
+        model's device). Every prompt is sampled as :meth:`generate` samples it alone, up to and including
+        ``eos_token_id`` if that is drawn.
+
+        Requests share a paged KV cache (``cache``, or one made for at most ``max_batch`` requests at a time):
+        prompts wait until a row and pages for their longest continuation are free, new prompts are
+        processed packed in one row, and all running requests decode together. On CUDA the decoding step
+        is captured once in a CUDA graph: lengths, tables and slots are advanced on the device, so the
+        same graph serves every step."""
+        self.eval()
+        dev = self.tok_embeddings.weight.device
+        seqs = [torch.as_tensor(p, dtype=torch.int64).tolist() for p in prompts]
+        if any(not s or len(s) > self.config.seq_length for s in seqs):
+            raise ValueError(f"prompts must have 1 to {self.config.seq_length} tokens")
+        # as in generate(): the last token drawn is never cached, so it may lie one past seq_length
+        limits = [min(max_new_tokens, self.config.seq_length - len(s) + 1) for s in seqs]
+        waiting = [i for i, n in enumerate(limits) if n > 0]
+        if cache is None and waiting:
+            attn = self.blocks[0].gqa
+            dt = compute_dtype(self.tok_embeddings.weight)
+            span = [len(seqs[i]) + limits[i] - 1 for i in waiting]
+            rows = min(max_batch, len(waiting))
+            pages = sum(sorted((n + page_size - 1) // page_size for n in span)[-rows:])
+            cache = PagedKVCache(len(self.blocks), pages, page_size, attn.n_kv_heads, attn.head_dim, rows, max(span), dt, dev)
+        for i in waiting:
+            span = len(seqs[i]) + limits[i] - 1
+            if span > cache.max_seq_len or cache.pages_for(span) > cache.n_pages:
+                raise ValueError(f"the cache is too small for a prompt of {len(seqs[i])} tokens and its continuation")
+        decoder = None
+        running: dict[int, int] = {}  # cache row -> prompt
+        reserved: dict[int, int] = {}  # cache row -> pages of its longest continuation
+        out = [list(s) for s in seqs]
+
+        def finished(row: int) -> bool:
+            i = running[row]
+            return len(out[i]) - len(seqs[i]) >= limits[i] or (eos_token_id is not None and out[i][-1] == eos_token_id)
+
+        def retire() -> None:
+            done = [row for row in running if finished(row)]
+            if done:
+                cache.release(done)
+                for row in done:
+                    del running[row], reserved[row]
+
+        while waiting or running:
+            admitted: list[int] = []
+            capacity = cache.n_free_pages + sum(cache.pages_for(cache.lens[r]) for r in running)
+            for row in range(cache.max_batch):
+                if not waiting or row in running or cache.lens[row]:
+                    continue
+                i = waiting[0]
+                need = cache.pages_for(len(seqs[i]) + limits[i] - 1)
+                if need + sum(reserved.values()) > capacity:
+                    break
+                running[row], reserved[row] = waiting.pop(0), need
+                admitted.append(row)
+            if not running:
+                raise ValueError("other requests of the cache leave no room")
+            if admitted:
+                counts = [len(seqs[running[r]]) if r in admitted else 0 for r in range(cache.max_batch)]
+                step = cache.plan(counts)
+                packed = torch.tensor([t for r in admitted for t in seqs[running[r]]]).to(dev)[None]
+                logits = self(packed, kv_caches=step.layers, select=step.plan.ends[admitted].long() - 1)
+                for row, t in zip(admitted, _sample(logits[0].float(), temperature, top_k, top_p).flatten().tolist()):
+                    out[running[row]].append(t)
+                retire()
+            if running:
+                if decoder is None:
+                    decoder = _Decoder(self, cache, cuda_graph=cuda_graph)
+                order = sorted(running)
+                logits = decoder.step(order, [out[running[r]][-1] for r in order])
+                for row, t in zip(order, _sample(logits, temperature, top_k, top_p).flatten().tolist()):
+                    out[running[row]].append(t)
+                retire()
+        return [torch.tensor(o, dtype=torch.int64, device=dev) for o in out]
 
     def get_num_params(self, *, non_embedding: bool = True) -> int:
         n = sum(p.numel() for p in self.parameters())
         if non_embedding:
             n -= self.tok_embeddings.weight.numel()
         return n
+
+
+def _sample(logits: torch.Tensor, temperature: float, top_k: int | None, top_p: float | None) -> torch.Tensor:
+    """Next tokens ``[B, 1]`` from fp32 ``logits`` ``[B, V]`` (changed in place); greedy at temperature 0."""
+    if temperature == 0:
+        return logits.argmax(dim=-1, keepdim=True)
+    logits = logits / temperature
+    if top_k is not None:
+        v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
+        logits[logits < v[:, [-1]]] = -float("inf")
+    if top_p is not None:
+        sorted_logits, sorted_idx = torch.sort(logits, descending=True)
+        cum = torch.cumsum(torch.softmax(sorted_logits, dim=-1), dim=-1)
+        remove = cum > top_p
+        remove[..., 1:] = remove[..., :-1].clone()
+        remove[..., 0] = False
+        logits[remove.scatter(1, sorted_idx, remove)] = -float("inf")
+    return torch.multinomial(torch.softmax(logits, dim=-1), num_samples=1)
+
+
+class _Decoder:
+    """Single-token steps of the running requests of a paged cache, padded to ``max_batch`` tokens. On one
+    CUDA GPU the second step is captured in a CUDA graph that all later steps replay."""
+
+    def __init__(self, model: Gemma, cache: PagedKVCache, *, cuda_graph: bool) -> None:
+        self.model, self.cache = model, cache
+        dev = cache.device
+        self.counts = torch.zeros(cache.max_batch, dtype=torch.int32, device=dev)
+        self.tokens = torch.zeros(1, cache.max_batch, dtype=torch.int64, device=dev)
+        self.use_graph = cuda_graph and dev.type == "cuda" and not tpc.active(model.tp) and model._before_forward is None
+        self.graph: torch.cuda.CUDAGraph | None = None
+        self.logits: torch.Tensor | None = None
+        self.steps = 0
+
+    def _run(self) -> torch.Tensor:
+        step = self.cache.plan_on_device(self.counts, self.cache.max_batch)
+        return self.model(self.tokens, kv_caches=step.layers)[0]
+
+    def step(self, rows: list[int], last: list[int]) -> torch.Tensor:
+        """fp32 logits ``[len(rows), V]`` after appending ``last[i]`` to the request in ``rows[i]`` (ascending)."""
+        counts = [0] * self.cache.max_batch
+        for r in rows:
+            counts[r] = 1
+        pad = self.cache.max_batch - len(rows)
+        self.counts.copy_(torch.tensor(counts, dtype=torch.int32))
+        self.tokens.copy_(torch.tensor([last + [0] * pad]))
+        if self.use_graph and self.steps == 1:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self.logits = self._run()
+            self.graph = graph
+        if self.graph is not None:
+            self.graph.replay()
+            logits = self.logits
+        else:
+            logits = self._run()
+        self.steps += 1
+        self.cache.advance(counts)
+        return logits[: len(rows)].float()
 
 
 def configure_optimizer(

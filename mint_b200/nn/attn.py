@@ -13,11 +13,13 @@ import torch
 from torch import nn
 
 from mint_b200.kvcache.base import KVCache
+from mint_b200.kvcache.paged import PagedLayer
 from mint_b200.nn.base import compute_dtype
 from mint_b200.nn.flashattn import FlashAttention
 from mint_b200.nn.norm import RMSNorm
-from mint_b200.nn.pos import PosEmbeddings, RoPE
+from mint_b200.nn.pos import ALiBiPositionalBias, NoPE, PosEmbeddings, RoPE
 from mint_b200.ops.linear import linear
+from mint_b200.ops.paged import paged_attention, qk_norm_rope_paged
 from mint_b200.ops.rope import qk_norm_rope
 from mint_b200.parallel import fused as fused_tp
 from mint_b200.parallel import tp as tpc
@@ -83,14 +85,53 @@ class GroupedQueryAttention(nn.Module):
         q, k, bias = self.pos_embeddings(q, k, start_pos=start_pos)
         return q, k, v, bias
 
+    def _forward_paged(self, x: torch.Tensor, layer: PagedLayer) -> torch.Tensor:
+        """One step over a paged cache: ``x`` [1, N, E] holds the packed tokens of ``layer.step``. Prompts whose
+        requests are new attend to each other as packed documents; other tokens attend over the pages."""
+        if x.shape[0] != 1:
+            raise ValueError(f"paged steps pack all tokens into one row, got a batch of {x.shape[0]}")
+        dt = compute_dtype(x)
+        x = tpc.enter_column_parallel(x, self.tp)
+        step, n = layer.step, x.shape[1]
+        pe = self.pos_embeddings
+        cos = sin = slopes = None
+        if isinstance(pe, RoPE):
+            cos, sin = pe.tables()
+        elif isinstance(pe, ALiBiPositionalBias):
+            first = self.tp.rank * self.n_heads if tpc.active(self.tp) else 0
+            slopes = pe.slopes.reshape(-1)[first : first + self.n_heads].float()
+        elif not isinstance(pe, NoPE):
+            raise ValueError(f"paged caches take rope, linear_rope, alibi or nope positions, not {type(pe).__name__}")
+        if all(type(m) is nn.Linear for m in (self.wq, self.wk, self.wv)):
+            qkv = linear(x, self.wq.weight, self.wk.weight, self.wv.weight, compute_dtype=dt)
+        else:
+            qkv = torch.cat([self.wq(x), self.wk(x), self.wv(x)], dim=-1)
+        packed = step.fresh and step.longest > 1 and slopes is None
+        out = qk_norm_rope_paged(
+            qkv.view(n, -1), self.n_heads, self.n_kv_heads, self.head_dim, self.q_norm.scale, self.k_norm.scale, cos, sin,
+            step.plan.positions, step.plan.slots, layer.k_pages, layer.v_pages, eps=self.q_norm.eps, return_kv=packed,
+        )
+        window = self.window_size if self.window_size > 0 else -1
+        if packed:
+            q, k, v = (t.unsqueeze(0) for t in out)
+            out = self.attention(q, k, v, causal=True, window_size=(window, -1), doc_ids=step.doc_ids)
+        else:
+            out = paged_attention(out, layer.k_pages, layer.v_pages, step.block_tables, step.plan.positions,
+                                  step.plan.rows, window_left=window, alibi_slopes=slopes)
+        out = out.reshape(1, n, -1)
+        y = linear(out, self.wo.weight, compute_dtype=dt) if type(self.wo) is nn.Linear else self.wo(out)
+        return tpc.exit_row_parallel(y, self.tp)
+
     def forward(
         self,
         x: torch.Tensor,
-        kv_cache: KVCache | None = None,
+        kv_cache: KVCache | PagedLayer | None = None,
         start_pos: int = 0,
         base_attn_mask: torch.Tensor | None = None,
         doc_ids: torch.Tensor | None = None,
     ) -> torch.Tensor:
+        if isinstance(kv_cache, PagedLayer):
+            return self._forward_paged(x, kv_cache)
         dt = compute_dtype(x)
         # TP on CUDA: QKV GEMM with its all-gather (SP) or backward all-reduce (no SP), wo GEMM with its
         # reduce-scatter (SP) or all-reduce (no SP), each as fused kernels
