@@ -6,7 +6,7 @@
 // share a KV head), at most 16 flops per byte for G = 16, so HBM bandwidth is the bound and the design is
 // about keeping enough bytes in flight on every SM whatever the lengths are.
 //
-// * Work is cut into tiles of 64 keys of one KV head (item = query x KV head). The kernel computes, from the
+// * Work is cut into tiles of 64 (or 128) keys of one KV head (item = query x KV head). The kernel computes, from the
 //   positions on the device, how many tiles there are and gives every CTA an equal contiguous share, so one
 //   request of any length, or a batch of mixed lengths, fills the GPU without a plan from the host (and a
 //   CUDA graph follows the lengths). A CTA whose share starts or ends inside an item leaves an fp32 partial
@@ -17,7 +17,7 @@
 //   swizzle, so the fragment loads are free of bank conflicts) into a ring of stages. Pages that hold no
 //   visible key are requested out of range: TMA fills zeros and reads nothing, and a corrupt table entry
 //   cannot read outside the pool.
-// * Four consumer warps take 16 keys of a tile each and keep their own running max, sum and output in
+// * Four consumer warps take 16 (32) keys of a tile each and keep their own running max, sum and output in
 //   registers, so there is no exchange until an item ends, when the warps' results are merged through the
 //   item's last stage. Products run on mma.sync m16n8k16 with the keys (S^T = K Q^T) and the output columns
 //   (O^T = V^T P^T) on the M side and 8 query rows per N block: a group of 1 to 8 query heads fills one block,
@@ -37,7 +37,10 @@
 namespace mint {
 namespace paged {
 
-constexpr int kTile = 64;          // keys per tile
+// Keys per tile: 64-wide heads take twice as many, since a tile's latencies do not shrink with its bytes
+// (64 requests of 4096 keys, 64 heads over 4, pages of 16: 57.9 us with tiles of 64, 54.4 us with 128).
+template <int D>
+constexpr int kTileOf = D == 64 ? 128 : 64;
 constexpr int kWarps = 4;          // consumer warps
 constexpr int kThreads = 32 * (kWarps + 2);  // and a producer warp each for K and V
 constexpr int kMinTiles = 1;       // a share is at least this many tiles
@@ -46,21 +49,23 @@ constexpr int kJoinWarps = 8;
 // NB blocks of 8 query rows per item; TWIN: one block whose columns 4-7 repeat rows 0-3 (hi / lo terms)
 template <int D, int NB>
 struct Config {
-  static constexpr int kRows = 8 * NB;  // query rows per item
+  static constexpr int kTile = kTileOf<D>;
+  static constexpr int kBlocks = kTile / (16 * kWarps);  // of 16 keys per warp
+  static constexpr int kRows = 8 * NB;                   // query rows per item
   static constexpr int kKvBytes = kTile * D * 2;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kStageBytes = (2 * kKvBytes + kQBytes + 1023) / 1024 * 1024;
-  // two CTAs per SM where three stages fit twice, else one
   static constexpr int kControl = 3072;  // scan, barriers, tile descriptions, merge statistics, base alignment
-  static constexpr int kHalf = 113 * 1024, kFull = 227 * 1024;
-  static constexpr bool kTwo = (kHalf - kControl) / kStageBytes >= 3;
-  static constexpr int kFit = ((kTwo ? kHalf : kFull) - kControl) / kStageBytes;
-  static constexpr int kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kSmSmem = 228 * 1024, kCtaSmem = 227 * 1024;
+  static constexpr int fit(int ctas) { return ((ctas > 1 ? kSmSmem / ctas - 1024 : kCtaSmem) - kControl) / kStageBytes; }
+  // two CTAs per SM where three stages fit twice, else one
+  static constexpr int kCtas = fit(2) >= 3 ? 2 : 1;
+  static constexpr int kStages = fit(kCtas) < 6 ? fit(kCtas) : 6;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
-  // the merge goes 16 rows at a time through a stage, lines padded against bank conflicts
-  static constexpr int kMergeRows = kRows < 16 ? kRows : 16, kMergeLine = D + 4;
-  static_assert(kStages >= 2 && kSmem + 1024 <= kFull, "shared memory");
-  static_assert(kWarps * kMergeRows * kMergeLine * 4 <= kStageBytes, "merge buffer");
+  static constexpr int kMergeLine = D + 4;  // lines of the merge buffer (a stage), padded against bank conflicts
+  static_assert(kStages >= 3 || D == 256, "stages");
+  static_assert(kStages >= 2 && kSmem + kControl - 1024 <= kCtaSmem, "shared memory");
+  static_assert(kWarps * kRows * kMergeLine * 4 <= kStageBytes, "merge buffer");
 };
 
 struct alignas(16) TileInfo {  // the tile in a stage, for the consumers
@@ -157,8 +162,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // Keys [lo, hi) that query n sees (hi = 0: none) and its table row.
 struct Span {
   int row, lo, hi, pos;
-  __device__ __forceinline__ int first() const { return lo / kTile; }
-  __device__ __forceinline__ int tiles() const { return hi > 0 ? (hi - 1) / kTile - lo / kTile + 1 : 0; }
+  template <int TILE>
+  __device__ __forceinline__ int tiles() const {
+    return hi > 0 ? (hi - 1) / TILE - lo / TILE + 1 : 0;
+  }
 };
 __device__ __forceinline__ Span span_of(const AttnParams& p, int row, int pos) {
   Span s{row, 0, 0, pos};
@@ -194,9 +201,10 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32
 }
 
 template <typename T, int D, int NB, bool TWIN>
-__global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, Config<D, NB>::kCtas)
     attend_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, AttnParams p) {
   using C = Config<D, NB>;
+  constexpr int kTile = C::kTile, KB = C::kBlocks;
   extern __shared__ uint8_t s_raw[];
   __shared__ uint64_t full[C::kStages], empty[C::kStages], merge;
   __shared__ TileInfo info[C::kStages];
@@ -213,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
   const int chunk = (p.N + kThreads - 1) / kThreads;
   const int n0 = min(p.N, tid * chunk), n1 = min(p.N, n0 + chunk);
   int inc = 0;
-  for (int n = n0; n < n1; ++n) inc += span_at(p, n).tiles();
+  for (int n = n0; n < n1; ++n) inc += span_at(p, n).template tiles<kTile>();
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 2);
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
       query = owner * chunk;
       if (chunk > 1) {
         while (true) {
-          int end = query + lane < p.N ? span_at(p, query + lane).tiles() : 0;
+          int end = query + lane < p.N ? span_at(p, query + lane).template tiles<kTile>() : 0;
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, end, d);
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
       Piece c{};
       while (left > 0) {
         c.s = span_at(p, query);
-        c.tiles = c.s.tiles();
+        c.tiles = c.s.template tiles<kTile>();
         if (off < c.tiles * per_query) break;
         ++query;
         off = 0;
@@ -300,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     auto entries = [&](const Span& s, int page) {
       return page + lane <= (s.pos >> p.page_shift) ? p.tables[s.row * p.tstride + page + lane] : -1;
     };
-    auto first_page = [&](const Piece& c) { return ((c.s.first() + c.at) * kTile) >> p.page_shift; };
+    auto first_page = [&](const Piece& c) { return ((c.s.lo / kTile + c.at) * kTile) >> p.page_shift; };
     const int box_lines = min(1 << p.page_shift, kTile), boxes = kTile / box_lines;
     const CUtensorMap* map = is_k ? &tk : &tv;
     int4 join = make_int4(0, 0, 0, 0);
@@ -328,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
       Piece nxt{};
       int ahead = -1, nxt_base = 0, nxt_entry = -1;
       for (int i = 0; i < cur.len; ++i) {
-        const int key0 = (cur.s.first() + cur.at + i) * kTile;
+        const int key0 = (cur.s.lo / kTile + cur.at + i) * kTile;
         const int page0 = key0 >> p.page_shift, line = key0 & ((1 << p.page_shift) - 1) & -box_lines;
         if (page0 >= base + 32) {
           base = page0;
@@ -407,14 +415,19 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     for (int i = tid; i < p.Hq * D / 8; i += 32 * kWarps) o[i] = make_uint4(0, 0, 0, 0);
   }
   // tile line r: 64-column parts of a box are half_stride bytes apart, 16-byte chunk c of a line sits at c ^ (r & 7)
-  const int box_shift = min(p.page_shift, 6), box_lines = 1 << box_shift;
+  const int box_shift = min(p.page_shift, kTile == 128 ? 7 : 6), box_lines = 1 << box_shift;
   const uint32_t half_stride = box_lines * 128;
   auto line_offset = [&](int r) { return static_cast<uint32_t>((r >> box_shift) * box_lines * D * 2 + (r & (box_lines - 1)) * 128); };
-  const uint32_t k_line = line_offset(warp * 16 + (lane & 15));
-  const uint32_t v_line = line_offset(warp * 16 + (lane & 7) + ((lane >> 4) << 3));
+  uint32_t k_line[KB], v_line[KB];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    const int r0 = (warp * KB + kb) * 16;
+    k_line[kb] = line_offset(r0 + (lane & 15));
+    v_line[kb] = line_offset(r0 + (lane & 7) + ((lane >> 4) << 3));
+  }
   const uint32_t k_chunk = (lane >> 4) ^ (lane & 7), v_chunk = ((lane >> 3) & 1) ^ (lane & 7);
   const uint32_t base_addr = smem_u32(stages);
-  const int my_key = warp * 16 + (lane >> 2);  // and + 8
+  const int my_key = warp * KB * 16 + (lane >> 2);  // and + 8, in each block of 16
   const int my_row = 2 * (lane & 3);           // and + 1, in each block of 8
 
   uint32_t qf[NB][D / 16][2];
@@ -453,46 +466,58 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
         }
       }
     }
-    // S^T = K Q^T: s[nb][0..1] = key my_key, rows my_row, + 1; s[nb][2..3] = key my_key + 8
-    float s[NB][4];
+    // S^T = K Q^T: s[kb][nb][0..1] = key my_key, rows my_row, + 1; s[kb][nb][2..3] = key my_key + 8
+    float s[KB][NB][4];
     {
-      float alt[NB][4];  // second chain of accumulators: halves the dependent products
+      float alt[KB][NB][4];  // second chain of accumulators: halves the dependent products
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nb][e] = alt[nb][e] = 0.f;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t kf[4];
-        ldsm4(kf, k_addr + k_line + (ks / 4) * half_stride + (((ks % 4) * 2) ^ k_chunk) * 16);
+          for (int e = 0; e < 4; ++e) s[kb][nb][e] = alt[kb][nb][e] = 0.f;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma16816<T>((ks & 1) ? alt[nb] : s[nb], kf, qf[nb][ks][0], qf[nb][ks][1]);
-      }
+      for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+        for (int kb = 0; kb < KB; ++kb) {
+          uint32_t kf[4];
+          ldsm4(kf, k_addr + k_line[kb] + (ks / 4) * half_stride + (((ks % 4) * 2) ^ k_chunk) * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nb][e] = (s[nb][e] + alt[nb][e]) * p.scale_log2;
+          for (int nb = 0; nb < NB; ++nb)
+            mma16816<T>((ks & 1) ? alt[kb][nb] : s[kb][nb], kf, qf[nb][ks][0], qf[nb][ks][1]);
+        }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[kb][nb][e] = (s[kb][nb][e] + alt[kb][nb][e]) * p.scale_log2;
     }
     if (p.slopes != nullptr) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s[nb][e] = fmaf(slope[nb][e & 1], static_cast<float>(t.key0 + my_key + (e >> 1) * 8 - t.pos), s[nb][e]);
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[kb][nb][e] = fmaf(slope[nb][e & 1], static_cast<float>(t.key0 + my_key + kb * 16 + (e >> 1) * 8 - t.pos),
+                                s[kb][nb][e]);
     }
     const bool edge = t.key0 < t.lo || t.key0 + kTile > t.hi;
     if (edge) {
 #pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const int key = t.key0 + my_key + e * 4;
-        if (key < t.lo || key >= t.hi) {
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) s[nb][e] = s[nb][e + 1] = -INFINITY;
+        for (int e = 0; e < 4; e += 2) {
+          const int key = t.key0 + my_key + kb * 16 + e * 4;
+          if (key < t.lo || key >= t.hi) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) s[kb][nb][e] = s[kb][nb][e + 1] = -INFINITY;
+          }
         }
-      }
       // a line outside the keys seen may hold anything (0 * NaN is NaN): clear the V lines this warp reads
-      for (int i = lane; i < 16 * (D / 8); i += 32) {
-        const int r = warp * 16 + i / (D / 8), c = i % (D / 8);
+      for (int i = lane; i < 16 * KB * (D / 8); i += 32) {
+        const int r = warp * KB * 16 + i / (D / 8), c = i % (D / 8);
         if (t.key0 + r < t.lo || t.key0 + r >= t.hi)
           asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_addr + line_offset(r) + (c / 8) * half_stride +
                                                                        (c % 8) * 16),
@@ -508,7 +533,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float mx = fmaxf(s[nb][c], s[nb][2 + c]);
+        float mx = fmaxf(s[0][nb][c], s[0][nb][2 + c]);
+#pragma unroll
+        for (int kb = 1; kb < KB; ++kb) mx = fmaxf(mx, fmaxf(s[kb][nb][c], s[kb][nb][2 + c]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const float next = fmaxf(m[nb][c], mx);
@@ -516,9 +543,14 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
         fix[nb][c] = exp2f(m[nb][c] - base);
         moved |= next != m[nb][c];
         m[nb][c] = next;
-        s[nb][c] = exp2f(s[nb][c] - base);
-        s[nb][2 + c] = exp2f(s[nb][2 + c] - base);
-        l[nb][c] = fmaf(l[nb][c], fix[nb][c], s[nb][c] + s[nb][2 + c]);
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          s[kb][nb][c] = exp2f(s[kb][nb][c] - base);
+          s[kb][nb][2 + c] = exp2f(s[kb][nb][2 + c] - base);
+          sum += s[kb][nb][c] + s[kb][nb][2 + c];
+        }
+        l[nb][c] = fmaf(l[nb][c], fix[nb][c], sum);
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -529,32 +561,36 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
           for (int e = 0; e < 4; ++e) o[nb][i][e] *= fix[nb][e & 1];
     }
     // O^T += V^T P^T; P^T's operand layout is the transpose of S^T's
-    uint32_t hi[NB][2], lo[NB][2];
+    uint32_t hi[KB][NB][2], lo[KB][NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t a, b;
-        split2<T>(s[nb][2 * h], s[nb][2 * h + 1], a, b);
-        if (TWIN) {
-          hi[nb][h] = transpose8((lane & 2) ? b : a);  // columns 4-7 carry lo
-        } else {
-          hi[nb][h] = transpose8(a);
-          lo[nb][h] = transpose8(b);
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a, b;
+          split2<T>(s[kb][nb][2 * h], s[kb][nb][2 * h + 1], a, b);
+          if (TWIN) {
+            hi[kb][nb][h] = transpose8((lane & 2) ? b : a);  // columns 4-7 carry lo
+          } else {
+            hi[kb][nb][h] = transpose8(a);
+            lo[kb][nb][h] = transpose8(b);
+          }
+        }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        uint32_t vf[4];
+        ldsm4_t(vf, v_addr + v_line[kb] + (i / 4) * half_stride + (((i % 4) * 2) ^ v_chunk) * 16);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          mma16816<T>(o[nb][i], vf, hi[kb][nb][0], hi[kb][nb][1]);
+          if (!TWIN) mma16816<T>(o[nb][i], vf, lo[kb][nb][0], lo[kb][nb][1]);
         }
       }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      uint32_t vf[4];
-      ldsm4_t(vf, v_addr + v_line + (i / 4) * half_stride + (((i % 4) * 2) ^ v_chunk) * 16);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        mma16816<T>(o[nb][i], vf, hi[nb][0], hi[nb][1]);
-        if (!TWIN) mma16816<T>(o[nb][i], vf, lo[nb][0], lo[nb][1]);
-      }
-    }
     if (t.flags & 2) {
-      // merge the warps' results through this stage, 16 rows at a time
+      // merge the warps' results through this stage
       const int kv_head = t.group / p.groups, row0 = (t.group - kv_head * p.groups) * C::kRows;
       const int live_rows = min(C::kRows, p.G - row0);
       float* buf = reinterpret_cast<float*>(stages + stage * C::kStageBytes);
@@ -571,60 +607,55 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kTwo ? 2 : 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[0][i][e] += __shfl_xor_sync(0xffffffffu, o[0][i][e], 2);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&merge);  // done with this stage, and with what was merged before
+      if (!wait_warp(&merge, merge_phase, p.status, abort_flag)) return;
+      merge_phase ^= 1u;
 #pragma unroll
-      for (int mr = 0; mr < C::kRows; mr += C::kMergeRows) {
-        if (mr >= live_rows) break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&merge);  // done with this stage, and with what was merged before
-        if (!wait_warp(&merge, merge_phase, p.status, abort_flag)) return;
-        merge_phase ^= 1u;
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int nb = mr / 8; nb < (mr + C::kMergeRows) / 8; ++nb)
+        for (int c = 0; c < 2; ++c) {
+          const int row = nb * 8 + my_row + c;
+          if (row < live_rows) {
+            if (lane < 4) s_ml[warp][row] = make_float2(m[nb][c], l[nb][c]);
+            float* dst = buf + (warp * C::kRows + row) * C::kMergeLine + (lane >> 2);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int row = nb * 8 + my_row + c;
-            if (row < live_rows) {
-              if (lane < 4) s_ml[warp][row] = make_float2(m[nb][c], l[nb][c]);
-              float* dst = buf + (warp * C::kMergeRows + row - mr) * C::kMergeLine + (lane >> 2);
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) {
-                dst[i * 16] = o[nb][i][c];
-                dst[i * 16 + 8] = o[nb][i][2 + c];
-              }
+            for (int i = 0; i < D / 16; ++i) {
+              dst[i * 16] = o[nb][i][c];
+              dst[i * 16 + 8] = o[nb][i][2 + c];
             }
           }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&merge);
-        if (!wait_warp(&merge, merge_phase, p.status, abort_flag)) return;
-        merge_phase ^= 1u;
-        const int rows_here = min(C::kMergeRows, live_rows - mr);
-        for (int i = tid; i < rows_here * (D / 4); i += 32 * kWarps) {
-          const int r = i / (D / 4), row = mr + r, c = (i % (D / 4)) * 4;
-          float M = -INFINITY, L = 0.f;
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&merge);
+      if (!wait_warp(&merge, merge_phase, p.status, abort_flag)) return;
+      merge_phase ^= 1u;
+      for (int i = tid; i < live_rows * (D / 4); i += 32 * kWarps) {
+        const int row = i / (D / 4), c = (i % (D / 4)) * 4;
+        float M = -INFINITY, L = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w][row].x);
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w][row].x);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float2 ml = s_ml[w][row];
-            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-            const float4 y = *reinterpret_cast<const float4*>(buf + (w * C::kMergeRows + r) * C::kMergeLine + c);
-            L = fmaf(ml.y, f, L);
-            x.x = fmaf(y.x, f, x.x);
-            x.y = fmaf(y.y, f, x.y);
-            x.z = fmaf(y.z, f, x.z);
-            x.w = fmaf(y.w, f, x.w);
-          }
-          if (t.out < 0) {
-            const float inv = 1.f / L;
-            T* dst = static_cast<T*>(p.o) + (static_cast<long long>(t.query) * p.Hq + kv_head * p.G + row0 + row) * D + c;
-            T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
-            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
-          } else {
-            const long long at = static_cast<long long>(t.out) * p.part_rows + row;
-            *reinterpret_cast<float4*>(p.part_o + at * D + c) = x;
-            if (c == 0) p.part_ml[at] = make_float2(M, L);
-          }
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = s_ml[w][row];
+          const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+          const float4 y = *reinterpret_cast<const float4*>(buf + (w * C::kRows + row) * C::kMergeLine + c);
+          L = fmaf(ml.y, f, L);
+          x.x = fmaf(y.x, f, x.x);
+          x.y = fmaf(y.y, f, x.y);
+          x.z = fmaf(y.z, f, x.z);
+          x.w = fmaf(y.w, f, x.w);
+        }
+        if (t.out < 0) {
+          const float inv = 1.f / L;
+          T* dst = static_cast<T*>(p.o) + (static_cast<long long>(t.query) * p.Hq + kv_head * p.G + row0 + row) * D + c;
+          T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
+          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+        } else {
+          const long long at = static_cast<long long>(t.out) * p.part_rows + row;
+          *reinterpret_cast<float4*>(p.part_o + at * D + c) = x;
+          if (c == 0) p.part_ml[at] = make_float2(M, L);
         }
       }
       __syncwarp();
@@ -694,14 +725,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p) {
   }
 }
 
-CUtensorMap page_map(const at::Tensor& t, int dtype) {
+CUtensorMap page_map(const at::Tensor& t, int dtype, int tile) {
   // {64 columns, lines, D / 64 column parts, heads, pages}: one box is a page's lines of one head as
   // D / 64 parts of 128-byte rows
   const uint64_t D = t.size(3), lines = t.size(2);
   const uint64_t dims[5] = {64, lines, D / 64, static_cast<uint64_t>(t.size(1)), static_cast<uint64_t>(t.size(0))};
   auto stride = [&](int d) { return static_cast<uint64_t>(t.size(d) > 1 ? t.stride(d) : D); };
   const uint64_t strides[4] = {stride(2), 64, stride(1), stride(0)};
-  const uint32_t box[5] = {64, static_cast<uint32_t>(std::min<uint64_t>(lines, kTile)), static_cast<uint32_t>(D / 64), 1, 1};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(std::min<uint64_t>(lines, tile)), static_cast<uint32_t>(D / 64), 1, 1};
   return make_tmap_5d(t.data_ptr(), dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -717,7 +748,7 @@ void launch_attend(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, c
     MINT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     ready.fetch_or(1ull << device, std::memory_order_relaxed);
   }
-  const int grid = num_sms(device) * (C::kTwo ? 2 : 1);
+  const int grid = num_sms(device) * C::kCtas;
   p.groups = (p.G + C::kRows - 1) / C::kRows;
   p.part_rows = p.groups > 1 ? C::kRows : p.G;
   const int64_t slots = 2ll * grid * p.part_rows;
@@ -760,18 +791,17 @@ void launch_attend(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, c
   }
 }
 
-// Query rows per item: 4 (hi and lo terms side by side in one block of 8), 8, 16 or, where the outputs fit
-// the registers (heads up to 128), 32. Wider groups are several items, which read K and V again (from L2).
+// Query rows per item: 4 (hi and lo terms side by side in one block of 8), 8 or 16. Wider groups are several
+// items, which read K and V again (from L2 as far as it holds them): 32 rows at once leave registers for one
+// CTA per SM only and measured the same (256 requests of 4096 keys, 32 heads over 1: 204 us against 195).
 template <typename T, int D, typename... Args>
 void dispatch_rows(const AttnParams& p, Args&&... args) {
   if (p.G <= 4) {
     launch_attend<T, D, 1, true>(p, args...);
   } else if (p.G <= 8) {
     launch_attend<T, D, 1, false>(p, args...);
-  } else if (p.G <= 16 || D == 256) {
-    launch_attend<T, D, 2, false>(p, args...);
   } else {
-    launch_attend<T, D, D == 256 ? 2 : 4, false>(p, args...);
+    launch_attend<T, D, 2, false>(p, args...);
   }
 }
 
@@ -849,10 +879,11 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::
   p.window = static_cast<int>(std::max<int64_t>(-1, std::min<int64_t>(window, INT_MAX)));
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   const int type = dt == at::kBFloat16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUtensorMap tk = paged::page_map(kp, type), tv = paged::page_map(vp, type);
+  const int tile = D == 64 ? paged::kTileOf<64> : D == 128 ? paged::kTileOf<128> : paged::kTileOf<256>;
+  const CUtensorMap tk = paged::page_map(kp, type, tile), tv = paged::page_map(vp, type, tile);
   // the most tiles that a query can have; with one at most there is nothing to join
-  int64_t tiles_bound = std::max<int64_t>(1, (tables.size(1) * kp.size(2) + paged::kTile - 1) / paged::kTile);
-  if (window >= 0) tiles_bound = std::min<int64_t>(tiles_bound, window / paged::kTile + 2);
+  int64_t tiles_bound = std::max<int64_t>(1, (tables.size(1) * kp.size(2) + tile - 1) / tile);
+  if (window >= 0) tiles_bound = std::min<int64_t>(tiles_bound, window / tile + 2);
   const bool may_split = tiles_bound > 1;
   if (dt == at::kBFloat16) {
     paged::dispatch_dim<__nv_bfloat16>(p, D, tk, tv, q, may_split, tiles_bound, stream);
