@@ -83,10 +83,9 @@ inline void check_pool(const at::Tensor& t, const char* name, at::ScalarType dty
   MINT_CHECK(t.dim() == 4 && t.size(1) == n_kv && t.size(3) == D, name, " must be [pages, ", n_kv, ", page_size, ", D, "]");
   MINT_CHECK(t.scalar_type() == dtype, name, " must have the dtype of the queries (", dtype, ")");
   MINT_CHECK(t.size(0) >= 1 && t.size(0) < (1ll << 31), name, " has no pages");
-  MINT_CHECK(t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
-                 t.stride(0) > 0 && t.stride(1) > 0 && t.stride(2) > 0 &&
-                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-             name, " lines must be contiguous and 16-byte aligned");
+  bool lines = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int d = 0; d < 3; ++d) lines = lines && (t.size(d) == 1 || (t.stride(d) % 8 == 0 && t.stride(d) > 0));
+  MINT_CHECK(lines, name, " lines must be contiguous and 16-byte aligned");
   shift_of(t.size(2));
 }
 

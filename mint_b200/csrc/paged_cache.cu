@@ -371,7 +371,7 @@ std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fres
   for (const at::Tensor* t : {&seq, &fresh, static_cast<const at::Tensor*>(&tables), &free_pages, &free_head})
     MINT_CHECK(t->scalar_type() == at::kInt && t->device() == seq.device(), "paged_plan takes int32 tensors on one device");
   const int64_t B = seq.numel();
-  MINT_CHECK(fresh.numel() == B && tables.dim() == 2 && tables.size(0) == B && tables.stride(1) == 1,
+  MINT_CHECK(fresh.numel() == B && tables.dim() == 2 && tables.size(0) == B && (tables.size(1) <= 1 || tables.stride(1) == 1),
              "paged_plan: one length pair and one table row per request");
   MINT_CHECK(B <= paged::kMaxRequests, "paged_plan takes at most ", paged::kMaxRequests, " requests");
   MINT_CHECK(free_head.numel() == 1, "free_head has one element");

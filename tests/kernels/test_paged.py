@@ -222,6 +222,36 @@ def test_attention_offsets_beyond_32_bits():
     assert torch.equal(vp[pool - 1, :, 63], qkv.view(-1, dim)[8 + hkv :])
 
 
+@pytest.mark.parametrize("with_rows", [True, False])
+def test_attention_very_wide_tables(with_rows):
+    """Tables for 2^30 keys per request: the queries go in several launches so that tile numbers fit an int."""
+    page, n = 1024, 40
+    lens = [1 + 97 * i % 700 for i in range(4 if with_rows else n)]
+    kp, vp, tables, keys = make_cache(lens, 8, 64, page, torch.bfloat16)
+    wide = torch.zeros(len(lens), 2**20, dtype=torch.int32, device="cuda")
+    wide[:, : tables.shape[1]] = tables
+    rows = [i % 4 for i in range(n)] if with_rows else list(range(n))
+    pos = [lens[r] - 1 - i % min(3, lens[r]) for i, r in enumerate(rows)]
+    q = torch.randn(n, 16, 64, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    got = paged_attention(q.cuda(), kp, vp, wide, torch.tensor(pos, **i32), torch.tensor(rows, **i32) if with_rows else None)
+    want, mag = oracle(q, keys, pos, rows, -1, None, 1 / 8)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= U[torch.bfloat16] * want.abs() + 2.0**-11 * mag + 1e-7).all())
+
+
+def test_one_page_pools_with_odd_strides_of_single_dimensions():
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    flat = torch.randn(2, 8, 64, device="cuda", dtype=torch.bfloat16)
+    kp, vp = (flat[i].as_strided((1, 1, 8, 64), (3, 5, 64, 1)) for i in (0, 1))
+    q = torch.randn(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    one_column = torch.zeros(1, 3, **i32)[:, :1]
+    got = paged_attention(q, kp, vp, one_column, torch.tensor([4], **i32))
+    want, mag = oracle(q.cpu(), [(flat[0, :, None].cpu(), flat[1, :, None].cpu())], [4], [0], -1, None, 1 / 8)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= U[torch.bfloat16] * want.abs() + 2.0**-11 * mag + 1e-7).all())
+
+
 def test_attention_on_a_side_stream():
     kp, vp, tables, keys = make_cache([2000] * 4, 2, 128, 16, torch.bfloat16)
     q = torch.randn(4, 4, 128, device="cuda", dtype=torch.bfloat16)
