@@ -321,6 +321,8 @@ class Gemma(nn.Module):
         processed packed in one row, and all running requests decode together. On CUDA the decoding step
         is captured once in a CUDA graph: lengths, tables and slots are advanced on the device, so the
         same graph serves every step."""
+        if tpc.active(self.tp):
+            raise ValueError("generate_batch does not run under tensor parallelism")
         self.eval()
         dev = self.tok_embeddings.weight.device
         seqs = [torch.as_tensor(p, dtype=torch.int64).tolist() for p in prompts]
@@ -422,7 +424,7 @@ class _Decoder:
         dev = cache.device
         self.counts = torch.zeros(cache.max_batch, dtype=torch.int32, device=dev)
         self.tokens = torch.zeros(1, cache.max_batch, dtype=torch.int64, device=dev)
-        self.use_graph = cuda_graph and dev.type == "cuda" and not tpc.active(model.tp) and model._before_forward is None
+        self.use_graph = cuda_graph and dev.type == "cuda" and model._before_forward is None
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: torch.Tensor | None = None
         self.steps = 0

@@ -90,16 +90,16 @@ class GroupedQueryAttention(nn.Module):
         requests are new attend to each other as packed documents; other tokens attend over the pages."""
         if x.shape[0] != 1:
             raise ValueError(f"paged steps pack all tokens into one row, got a batch of {x.shape[0]}")
+        if tpc.active(self.tp):
+            raise ValueError("paged caches are not supported under tensor parallelism")
         dt = compute_dtype(x)
-        x = tpc.enter_column_parallel(x, self.tp)
         step, n = layer.step, x.shape[1]
         pe = self.pos_embeddings
         cos = sin = slopes = None
         if isinstance(pe, RoPE):
             cos, sin = pe.tables()
         elif isinstance(pe, ALiBiPositionalBias):
-            first = self.tp.rank * self.n_heads if tpc.active(self.tp) else 0
-            slopes = pe.slopes.reshape(-1)[first : first + self.n_heads].float()
+            slopes = pe.slopes.reshape(-1).float()
         elif not isinstance(pe, NoPE):
             raise ValueError(f"paged caches take rope, linear_rope, alibi or nope positions, not {type(pe).__name__}")
         if all(type(m) is nn.Linear for m in (self.wq, self.wk, self.wv)):
@@ -119,8 +119,7 @@ class GroupedQueryAttention(nn.Module):
             out = paged_attention(out, layer.k_pages, layer.v_pages, step.block_tables, step.plan.positions,
                                   step.plan.rows, window_left=window, alibi_slopes=slopes)
         out = out.reshape(1, n, -1)
-        y = linear(out, self.wo.weight, compute_dtype=dt) if type(self.wo) is nn.Linear else self.wo(out)
-        return tpc.exit_row_parallel(y, self.tp)
+        return linear(out, self.wo.weight, compute_dtype=dt) if type(self.wo) is nn.Linear else self.wo(out)
 
     def forward(
         self,

@@ -104,3 +104,18 @@ def test_model_refusals():
     step = PagedKVCache(2, 4, 8, 2, 16, max_batch=2, max_seq_len=16).plan([4, 4])
     with pytest.raises(ValueError, match="one row"), torch.no_grad():
         model(torch.zeros(2, 4, dtype=torch.int64), kv_caches=step.layers)
+
+
+def test_tensor_parallel_models_are_refused():
+    from mint_b200.parallel.tp import TPInfo
+
+    model = _model()
+    tp = TPInfo(**{"group": None, "rank": 0, "size": 2, "sp": False})
+    model.tp = tp
+    with pytest.raises(ValueError, match="tensor parallel"):
+        model.generate_batch(_prompts(4), 2)
+    model.tp = None
+    model.blocks[0].gqa.tp = tp
+    step = PagedKVCache(2, 4, 8, 2, 16, max_batch=1, max_seq_len=16).plan([4])
+    with pytest.raises(ValueError, match="tensor parallel"), torch.no_grad():
+        model(torch.zeros(1, 4, dtype=torch.int64), kv_caches=step.layers)
