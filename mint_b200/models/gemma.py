@@ -421,7 +421,7 @@ class _Decoder:
 
     def __init__(self, model: Gemma, cache: PagedKVCache, *, cuda_graph: bool) -> None:
         self.model, self.cache = model, cache
-        dev = cache.device
+        self.device = dev = cache.k_pages.device
         self.counts = torch.zeros(cache.max_batch, dtype=torch.int32, device=dev)
         self.tokens = torch.zeros(1, cache.max_batch, dtype=torch.int64, device=dev)
         self.use_graph = cuda_graph and dev.type == "cuda" and model._before_forward is None
@@ -433,6 +433,14 @@ class _Decoder:
         step = self.cache.plan_on_device(self.counts, self.cache.max_batch)
         return self.model(self.tokens, kv_caches=step.layers)[0]
 
+    def _capture(self) -> None:
+        """Capture on a stream of the cache's device: torch's default capture stream is on the device that was
+        current at the process's first capture, and kernels launched on another device would not be recorded."""
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=torch.cuda.Stream(self.device)):
+            self.logits = self._run()
+        self.graph = graph
+
     def step(self, rows: list[int], last: list[int]) -> torch.Tensor:
         """fp32 logits ``[len(rows), V]`` after appending ``last[i]`` to the request in ``rows[i]`` (ascending)."""
         counts = [0] * self.cache.max_batch
@@ -442,12 +450,10 @@ class _Decoder:
         self.counts.copy_(torch.tensor(counts, dtype=torch.int32))
         self.tokens.copy_(torch.tensor([last + [0] * pad]))
         if self.use_graph and self.steps == 1:
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                self.logits = self._run()
-            self.graph = graph
+            self._capture()
         if self.graph is not None:
-            self.graph.replay()
+            with torch.cuda.device(self.device):
+                self.graph.replay()
             logits = self.logits
         else:
             logits = self._run()
