@@ -23,9 +23,11 @@
 //   (O^T = V^T P^T) on the M side and 8 query rows per N block: a group of 1 to 8 query heads fills one block,
 //   where a tcgen05 tile (M = 128 query rows) would be 94 % padding and the tensor pipe is not the bound.
 // * Probabilities are split into two 16-bit terms, p = hi + lo, for the second product: they keep 16 bits of
-//   precision instead of bf16's 8. Groups of at most 4 heads get this for nothing: columns 4-7 of the N block
-//   repeat the rows, carry lo where columns 0-3 carry hi, and are added when the item ends. Scores, sums and
-//   outputs are fp32.
+//   precision instead of bf16's 8. fp16 has no exponents for small p: there both p and the running sum are
+//   2^15 times the probability relative to the running max, which puts the error of hi + lo below 2^-39 (16 bits
+//   for keys down to 15 nats under the max, 11 bits down to 19). Groups of at most 4 heads get the split for
+//   nothing: columns 4-7 of the N block repeat the rows, carry lo where columns 0-3 carry hi, and are added when
+//   the item ends. Scores, sums and outputs are fp32.
 //
 // Measured: 64 requests of 1024 to 32768 keys (16 heads over 4 of 128, pages of 16, 2.2 GB) 331 us, 6.7 TB/s, the
 // rate of a plain copy; the same with 8-line pages 90 % of it. Short work is bound by the chain of dependent reads
@@ -130,6 +132,12 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+// What probabilities (at most 1) are multiplied by before they are split; it cancels in the division by the sum.
+template <typename T>
+constexpr float kProbScale = 1.f;
+template <>
+constexpr float kProbScale<__half> = 32768.f;
 
 // (a, b) = hi + lo in two packed 16-bit pairs; lo holds what rounding to hi lost
 template <typename T>
@@ -552,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NB>::kCtas)
         float sum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          s[kb][nb][c] = exp2f(s[kb][nb][c] - base);
-          s[kb][nb][2 + c] = exp2f(s[kb][nb][2 + c] - base);
+          s[kb][nb][c] = exp2f(s[kb][nb][c] - base) * kProbScale<T>;
+          s[kb][nb][2 + c] = exp2f(s[kb][nb][2 + c] - base) * kProbScale<T>;
           sum += s[kb][nb][c] + s[kb][nb][2 + c];
         }
         l[nb][c] = fmaf(l[nb][c], fix[nb][c], sum);
