@@ -24,8 +24,8 @@
 //   where a tcgen05 tile (M = 128 query rows) would be 94 % padding and the tensor pipe is not the bound.
 // * Probabilities are split into two 16-bit terms, p = hi + lo, for the second product: they keep 16 bits of
 //   precision instead of bf16's 8. fp16 has no exponents for small p: there both p and the running sum are
-//   2^15 times the probability relative to the running max, which puts the error of hi + lo below 2^-39 (16 bits
-//   for keys down to 15 nats under the max, 11 bits down to 19). Groups of at most 4 heads get the split for
+//   2^15 times the probability relative to the running max, which puts the error of hi + lo below 2^-38 (16 bits
+//   for keys down to 15 nats under the max, 11 bits down to 18). Groups of at most 4 heads get the split for
 //   nothing: columns 4-7 of the N block repeat the rows, carry lo where columns 0-3 carry hi, and are added when
 //   the item ends. Scores, sums and outputs are fp32.
 //
@@ -139,22 +139,36 @@ constexpr float kProbScale = 1.f;
 template <>
 constexpr float kProbScale<__half> = 32768.f;
 
-// (a, b) = hi + lo in two packed 16-bit pairs; lo holds what rounding to hi lost
+// (a, b) = hi + lo in two packed 16-bit pairs: hi is rounded toward zero, so that lo, what that lost, is never
+// negative, and neither is below the smallest step of its type's grid (2^-126, or 2^-24 of fp16's 2^15): 0 times an
+// infinite value would be NaN, and a lo of the other sign would turn infinity into NaN. The floor adds nothing where
+// keys are masked (their values are zeroed) and at most 2^-39 of the largest probability to each term elsewhere.
+__device__ __forceinline__ uint32_t at_least(uint32_t x, __nv_bfloat162 least) {
+  const __nv_bfloat162 y = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x), least);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t at_least(uint32_t x, __half2 least) {
+  const __half2 y = __hmax2_nan(*reinterpret_cast<const __half2*>(&x), least);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
 template <typename T>
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo);
 template <>
 __device__ __forceinline__ void split2<__nv_bfloat16>(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16x2(a, b);
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
   const float2 f = bf16x2_to_float2(hi);
-  lo = pack_bf16x2(a - f.x, b - f.y);
+  const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x0080), __ushort_as_bfloat16(0x0080));
+  lo = at_least(pack_bf16x2(a - f.x, b - f.y), least);
+  hi = at_least(hi, least);
 }
 template <>
 __device__ __forceinline__ void split2<__half>(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  const __half2 least = __halves2half2(__ushort_as_half(1), __ushort_as_half(1));
   const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+  lo = at_least(*reinterpret_cast<const uint32_t*>(&l), least);
+  hi = at_least(hi, least);
 }
 
 __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, uint64_t* bar, int line, int head, int page) {

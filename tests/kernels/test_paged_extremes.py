@@ -1,8 +1,10 @@
-"""Paged attention at the ends of its ranges: fp16 weights far below the largest.
+"""Paged attention at the ends of its ranges: fp16 weights far below the largest, infinite values.
 
 Tolerances. As for ordinary inputs (tests/kernels/test_paged.py): one rounding to the output type (half of its eps
 times |out|; half of the smallest subnormal, 2^-25, where an fp16 output is subnormal) and 2^-11 of sum p|v|. The
 scores here are single products of fp16 numbers and exact, at most 18 below the largest: exp(-18) is above 2^-26."""
+
+import math
 
 import pytest
 import torch
@@ -64,3 +66,21 @@ def test_fp16_weights_far_below_the_largest(dim, hq, hkv, below):
     tol = U[torch.float16] * want.abs() + 2.0**-25 + 2.0**-11 * mag
     worst = ((got - want).abs() / mag).max().item()
     assert bool(((got - want).abs() <= tol).all()), f"off by {worst:.3g} of sum p|v|"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+@pytest.mark.parametrize("n,at", [(1, 0), (64, 3), (200, 199), (1500, 700)])
+def test_infinite_values_stay_infinite(dtype, hq, hkv, n, at):
+    """An infinite value that a query sees makes its column infinite and no other."""
+    g = torch.Generator().manual_seed(n)
+    dim = 128
+    k, v = (torch.randn(n, hkv, dim, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(1, hq, dim, generator=g).to(dtype)
+    want, mag = _oracle(q, k, v, dim**-0.5)
+    v[at, :, 5], v[at, :, 64] = math.inf, -math.inf
+    got = _call(q, k, v, dim**-0.5).double()
+    assert bool((got[..., 5] == math.inf).all()) and bool((got[..., 64] == -math.inf).all())
+    rest = [c for c in range(dim) if c not in (5, 64)]
+    err = (got - want).abs()[..., rest]
+    assert bool((err <= U[dtype] * want.abs()[..., rest] + 2.0**-11 * mag[..., rest] + 1e-7).all())
