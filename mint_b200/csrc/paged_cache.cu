@@ -5,6 +5,7 @@
 // line s % page_size of page s / page_size. Page sizes are powers of two. The reference has a dense
 // [B, Tmax, Hkv, D] cache only (mint/kvcache/base.py:4-65).
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "paged.cuh"
@@ -163,6 +164,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p) {
   }
   if (gtid == 0) *p.head_out = head + min(page_sum, left);
   if (bad) record_status(p.status, kStatusBadArgument);
+}
+
+constexpr int plan_smem(int64_t requests) { return static_cast<int>(2 * (requests + 1) * sizeof(int)); }
+
+// Raises the kernel's dynamic shared-memory limit to what kMaxRequests take, once per device: the default of 48 KB
+// includes the kernel's static arrays, and a limit set for one call could be lowered by another thread's.
+void allow_plan_smem(int device) {
+  static std::atomic<uint64_t> ready{0};
+  if (ready.load(std::memory_order_relaxed) >> device & 1) return;
+  check_smem_optin(plan_smem(kMaxRequests), device, "paged_plan");
+  MINT_CUDA_CHECK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan_smem(kMaxRequests)));
+  ready.fetch_or(1ull << device, std::memory_order_relaxed);
 }
 
 struct AppendParams {
@@ -404,11 +417,8 @@ std::vector<at::Tensor> paged_plan(const at::Tensor& seq, const at::Tensor& fres
   p.N = static_cast<int>(n_tokens);
   p.n_free = static_cast<int>(free_pages.numel());
   p.page_shift = paged::shift_of(page_size);
-  const int smem = static_cast<int>(2 * (B + 1) * sizeof(int));
-  if (smem > 48 * 1024) {
-    check_smem_optin(smem, seq.device().index(), "paged_plan");
-    MINT_CUDA_CHECK(cudaFuncSetAttribute(paged::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  }
+  const int smem = paged::plan_smem(B);
+  paged::allow_plan_smem(seq.device().index());
   const int64_t work = std::max<int64_t>(n_tokens, B);
   const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>((work + 1023) / 1024, 1), num_sms(seq.device().index())));
   paged::plan_kernel<<<grid, paged::kPlanThreads, smem, stream>>>(p);
