@@ -69,6 +69,11 @@ inline void check_inference(const char* op, std::initializer_list<const at::Tens
     MINT_CHECK(!t->requires_grad(), op, " has no gradient; call it under torch.no_grad()");
 }
 
+// the kernels read it 16 bytes at a time (rows of a contiguous tensor whose lines are multiples of 16 bytes)
+inline void check_vec16(const at::Tensor& t, const char* name) {
+  MINT_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
+}
+
 // log2 of a page size; the caches take powers of two from 8 (one 8-row swizzle group of a TMA box) up
 inline int shift_of(int64_t page_size) {
   MINT_CHECK(page_size >= 8 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,

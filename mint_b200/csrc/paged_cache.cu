@@ -454,6 +454,8 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
              "positions and slots are int32, one per token");
   MINT_CHECK(qs.scalar_type() == at::kFloat && ks.scalar_type() == at::kFloat && qs.numel() == D && ks.numel() == D,
              "norm scales are fp32 [head_dim]");
+  paged::check_vec16(qs, "q_scale");
+  paged::check_vec16(ks, "k_scale");
   paged::check_pool(kp, "k_pages", dt, n_kv, D);
   paged::check_pool(vp, "v_pages", dt, n_kv, D);
   MINT_CHECK(kp.sizes() == vp.sizes(), "k_pages and v_pages have different shapes");
@@ -465,8 +467,10 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
     check_contig(*cos_t, "cos");
     check_contig(*sin_t, "sin");
     MINT_CHECK(cos_t->scalar_type() == at::kFloat && sin_t->scalar_type() == at::kFloat && cos_t->dim() == 2 &&
-                   cos_t->size(1) == D / 2 && cos_t->sizes() == sin_t->sizes(),
-               "cos / sin are fp32 [positions, head_dim / 2]");
+                   cos_t->size(0) >= 1 && cos_t->size(1) == D / 2 && cos_t->sizes() == sin_t->sizes(),
+               "cos / sin are fp32 [positions, head_dim / 2] with one position at least");
+    paged::check_vec16(*cos_t, "cos");
+    paged::check_vec16(*sin_t, "sin");
     MINT_CHECK(cos_t->device() == qkv.device() && sin_t->device() == qkv.device(), "qk_norm_rope_paged takes tensors on one device");
     p.cos_t = cos_t->data_ptr<float>();
     p.sin_t = sin_t->data_ptr<float>();
