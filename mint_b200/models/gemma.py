@@ -31,6 +31,7 @@ from mint_b200.nn.norm import RMSNorm
 from mint_b200.ops.cross_entropy import lm_head_cross_entropy, lm_head_token_logps
 from mint_b200.ops.embedding import embedding
 from mint_b200.ops.linear import linear
+from mint_b200.ops.paged import has_kernels
 from mint_b200.parallel import fused as fused_tp
 from mint_b200.parallel import tp as tpc
 from mint_b200.utils.logger import logger
@@ -319,8 +320,8 @@ class Gemma(nn.Module):
         Requests share a paged KV cache (``cache``, or one made for at most ``max_batch`` requests at a time):
         prompts wait until a row and pages for their longest continuation are free, new prompts are
         processed packed in one row, and all running requests decode together. On CUDA the decoding step
-        is captured once in a CUDA graph: lengths, tables and slots are advanced on the device, so the
-        same graph serves every step."""
+        of a model that the paged kernels take (bf16 / fp16, heads of 64, 128 or 256) is captured once in a
+        CUDA graph: lengths, tables and slots are advanced on the device, so the same graph serves every step."""
         if tpc.active(self.tp):
             raise ValueError("generate_batch does not run under tensor parallelism")
         self.eval()
@@ -417,14 +418,17 @@ def _sample(logits: torch.Tensor, temperature: float, top_k: int | None, top_p: 
 
 class _Decoder:
     """Single-token steps of the running requests of a paged cache, padded to ``max_batch`` tokens. On one
-    CUDA GPU the second step is captured in a CUDA graph that all later steps replay."""
+    CUDA GPU, with a cache that the paged kernels take (bf16 / fp16, heads of 64, 128 or 256), the second step is
+    captured in a CUDA graph that all later steps replay."""
 
     def __init__(self, model: Gemma, cache: PagedKVCache, *, cuda_graph: bool) -> None:
         self.model, self.cache = model, cache
         self.device = dev = cache.k_pages.device
         self.counts = torch.zeros(cache.max_batch, dtype=torch.int32, device=dev)
         self.tokens = torch.zeros(1, cache.max_batch, dtype=torch.int64, device=dev)
-        self.use_graph = cuda_graph and dev.type == "cuda" and model._before_forward is None
+        # the PyTorch forms of the paged operators read lengths on the host, which a capture cannot record
+        kernels = has_kernels(cache.dtype, cache.k_pages.shape[-1])
+        self.use_graph = cuda_graph and dev.type == "cuda" and kernels and model._before_forward is None
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: torch.Tensor | None = None
         self.steps = 0

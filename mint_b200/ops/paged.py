@@ -46,6 +46,11 @@ class PagedPlan(NamedTuple):
     free_head: torch.Tensor
 
 
+def has_kernels(dtype: torch.dtype, head_dim: int) -> bool:
+    """Whether append and attention of CUDA tensors run kernels, which never wait for the host, or PyTorch code."""
+    return _ext.kernels_enabled() and dtype in _KERNEL_DTYPES and head_dim in _HEAD_DIMS
+
+
 def _inference_only(op: str, *tensors: torch.Tensor | None) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"mint_b200: {op} has no gradient; call it under torch.no_grad()")

@@ -61,3 +61,28 @@ def test_capture_and_replay_are_on_the_caches_device(fake_cuda):
     assert len(fake_cuda["graphs"]) == 1 and fake_cuda["replays"] == 3
     _, kw, devices = fake_cuda["graphs"][0]
     assert kw["stream"] == ("stream", torch.device("cuda", 1)) and devices == [torch.device("cuda", 1)]
+
+
+@pytest.mark.parametrize("dtype,head_dim,kernels,graph", [
+    (torch.bfloat16, 128, "on", True), (torch.float16, 64, "on", True), (torch.bfloat16, 256, "on", True),
+    (torch.float32, 128, "on", False), (torch.bfloat16, 32, "on", False), (torch.bfloat16, 96, "on", False),
+    (torch.bfloat16, 128, "off", False),
+])
+def test_only_steps_of_kernels_are_captured(dtype, head_dim, kernels, graph, monkeypatch):
+    """The PyTorch forms synchronize, which ends a capture with an error."""
+    monkeypatch.setenv("MINT_DISABLE_KERNELS", "1" if kernels == "off" else "0")
+
+    class Pages:  # stands for a CUDA tensor
+        device, shape = torch.device("cuda", 0), (1, 1, 1, 8, head_dim)
+
+    class Cache:
+        device, k_pages, max_batch = torch.device("cuda", 0), Pages, 2
+
+    Cache.dtype = dtype
+    monkeypatch.setattr(torch, "zeros", lambda *a, **k: None)
+    assert gemma._Decoder(_model_stub(), Cache, cuda_graph=True).use_graph == graph
+    assert not gemma._Decoder(_model_stub(), Cache, cuda_graph=False).use_graph
+
+
+def _model_stub():
+    return type("Stub", (), {"_before_forward": None})()
