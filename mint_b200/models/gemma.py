@@ -359,36 +359,40 @@ class Gemma(nn.Module):
                 for row in done:
                     del running[row], reserved[row]
 
-        while waiting or running:
-            admitted: list[int] = []
-            capacity = cache.n_free_pages + sum(cache.pages_for(cache.lens[r]) for r in running)
-            for row in range(cache.max_batch):
-                if not waiting or row in running or cache.lens[row]:
-                    continue
-                i = waiting[0]
-                need = cache.pages_for(len(seqs[i]) + limits[i] - 1)
-                if need + sum(reserved.values()) > capacity:
-                    break
-                running[row], reserved[row] = waiting.pop(0), need
-                admitted.append(row)
-            if not running:
-                raise ValueError("other requests of the cache leave no room")
-            if admitted:
-                counts = [len(seqs[running[r]]) if r in admitted else 0 for r in range(cache.max_batch)]
-                step = cache.plan(counts)
-                packed = torch.tensor([t for r in admitted for t in seqs[running[r]]]).to(dev)[None]
-                logits = self(packed, kv_caches=step.layers, select=step.plan.ends[admitted].long() - 1)
-                for row, t in zip(admitted, _sample(logits[0].float(), temperature, top_k, top_p).flatten().tolist()):
-                    out[running[row]].append(t)
-                retire()
+        try:
+            while waiting or running:
+                admitted: list[int] = []
+                capacity = cache.n_free_pages + sum(cache.pages_for(cache.lens[r]) for r in running)
+                for row in range(cache.max_batch):
+                    if not waiting or row in running or cache.lens[row]:
+                        continue
+                    i = waiting[0]
+                    need = cache.pages_for(len(seqs[i]) + limits[i] - 1)
+                    if need + sum(reserved.values()) > capacity:
+                        break
+                    running[row], reserved[row] = waiting.pop(0), need
+                    admitted.append(row)
+                if not running:
+                    raise ValueError("other requests of the cache leave no room")
+                if admitted:
+                    counts = [len(seqs[running[r]]) if r in admitted else 0 for r in range(cache.max_batch)]
+                    step = cache.plan(counts)
+                    packed = torch.tensor([t for r in admitted for t in seqs[running[r]]]).to(dev)[None]
+                    logits = self(packed, kv_caches=step.layers, select=step.plan.ends[admitted].long() - 1)
+                    for row, t in zip(admitted, _sample(logits[0].float(), temperature, top_k, top_p).flatten().tolist()):
+                        out[running[row]].append(t)
+                    retire()
+                if running:
+                    if decoder is None:
+                        decoder = _Decoder(self, cache, cuda_graph=cuda_graph)
+                    order = sorted(running)
+                    logits = decoder.step(order, [out[running[r]][-1] for r in order])
+                    for row, t in zip(order, _sample(logits, temperature, top_k, top_p).flatten().tolist()):
+                        out[running[row]].append(t)
+                    retire()
+        finally:  # left by an error: the rows and pages go back to the cache all the same
             if running:
-                if decoder is None:
-                    decoder = _Decoder(self, cache, cuda_graph=cuda_graph)
-                order = sorted(running)
-                logits = decoder.step(order, [out[running[r]][-1] for r in order])
-                for row, t in zip(order, _sample(logits, temperature, top_k, top_p).flatten().tolist()):
-                    out[running[row]].append(t)
-                retire()
+                cache.release(list(running))
         return [torch.tensor(o, dtype=torch.int64, device=dev) for o in out]
 
     def get_num_params(self, *, non_embedding: bool = True) -> int:
