@@ -28,6 +28,7 @@ from mint_b200.kvcache.paged import PagedKVCache, PagedLayer
 from mint_b200.nn.base import ModelConfig, compute_dtype
 from mint_b200.nn.blocks import GQAGluBlock
 from mint_b200.nn.norm import RMSNorm
+from mint_b200.ops import _ext
 from mint_b200.ops.cross_entropy import lm_head_cross_entropy, lm_head_token_logps
 from mint_b200.ops.embedding import embedding
 from mint_b200.ops.linear import linear
@@ -321,7 +322,8 @@ class Gemma(nn.Module):
         prompts wait until a row and pages for their longest continuation are free, new prompts are
         processed packed in one row, and all running requests decode together. On CUDA the decoding step
         of a model that the paged kernels take (bf16 / fp16, heads of 64, 128 or 256) is captured once in a
-        CUDA graph: lengths, tables and slots are advanced on the device, so the same graph serves every step."""
+        CUDA graph: lengths, tables and slots are advanced on the device, so the same graph serves every step.
+        Raises :class:`~mint_b200.ops._ext.DeviceStatusError` if a kernel reported an error."""
         if tpc.active(self.tp):
             raise ValueError("generate_batch does not run under tensor parallelism")
         self.eval()
@@ -393,6 +395,9 @@ class Gemma(nn.Module):
         finally:  # left by an error: the rows and pages go back to the cache all the same
             if running:
                 cache.release(list(running))
+        if dev.type == "cuda":  # the kernels' only report of a wait given up or an argument out of range
+            with torch.cuda.device(dev):
+                _ext.check_device_status()
         return [torch.tensor(o, dtype=torch.int64, device=dev) for o in out]
 
     def get_num_params(self, *, non_embedding: bool = True) -> int:
