@@ -81,7 +81,7 @@ class PagedKVCache:
             raise ValueError(f"KV cache overflow: {need} pages needed, {self._free} of {self.n_pages} free")
         fresh = all(b == 0 for b, n in zip(self.lens, new_lens) if n > 0)
         step = self.plan_on_device(torch.tensor(new_lens, dtype=torch.int32).to(self.device, non_blocking=True), n_tokens)
-        step.fresh, step.longest = fresh, max(new_lens)
+        step.fresh, step.new_lens = fresh, new_lens
         self.lens, self._free = after, self._free - need
         return step
 
@@ -137,5 +137,5 @@ class PagedStep:
         self.doc_ids = plan.rows.unsqueeze(0)  # the requests as documents of the packed row
         self.block_tables = cache.block_tables
         self.fresh = False  # every request with new tokens had none before
-        self.longest = 1  # most new tokens of a request, as far as the host knows
+        self.new_lens: list[int] = []  # new tokens of every request, if the host knows them
         self.layers = [PagedLayer(cache.k_pages[i], cache.v_pages[i], self) for i in range(cache.n_layers)]

@@ -18,8 +18,9 @@ from mint_b200.nn.base import compute_dtype
 from mint_b200.nn.flashattn import FlashAttention
 from mint_b200.nn.norm import RMSNorm
 from mint_b200.nn.pos import ALiBiPositionalBias, NoPE, PosEmbeddings, RoPE
+from mint_b200.ops.attention import has_kernel
 from mint_b200.ops.linear import linear
-from mint_b200.ops.paged import paged_attention, qk_norm_rope_paged
+from mint_b200.ops.paged import has_kernels, paged_attention, qk_norm_rope_paged
 from mint_b200.ops.rope import qk_norm_rope
 from mint_b200.parallel import fused as fused_tp
 from mint_b200.parallel import tp as tpc
@@ -86,8 +87,12 @@ class GroupedQueryAttention(nn.Module):
         return q, k, v, bias
 
     def _forward_paged(self, x: torch.Tensor, layer: PagedLayer) -> torch.Tensor:
-        """One step over a paged cache: ``x`` [1, N, E] holds the packed tokens of ``layer.step``. Prompts whose
-        requests are new attend to each other as packed documents; other tokens attend over the pages."""
+        """One step over a paged cache: ``x`` [1, N, E] holds the packed tokens of ``layer.step``.
+
+        When every request of the step is new, its prompts need not read the pages: they are the documents of one
+        packed row where the FlashAttention kernel takes them. Heads and types that only the paged kernel takes,
+        ALiBi models, and steps with older requests attend over the pages. What neither kernel takes (and CPU
+        tensors) attends prompt by prompt, so that no mask spans prompts that do not see each other."""
         if x.shape[0] != 1:
             raise ValueError(f"paged steps pack all tokens into one row, got a batch of {x.shape[0]}")
         if tpc.active(self.tp):
@@ -106,15 +111,25 @@ class GroupedQueryAttention(nn.Module):
             qkv = linear(x, self.wq.weight, self.wk.weight, self.wv.weight, compute_dtype=dt)
         else:
             qkv = torch.cat([self.wq(x), self.wk(x), self.wv(x)], dim=-1)
-        packed = step.fresh and step.longest > 1 and slopes is None
+        dense = x.is_cuda and has_kernel(qkv.dtype, self.head_dim)
+        prompts = step.fresh and max(step.new_lens, default=0) > 1 and slopes is None
+        if prompts and not dense and x.is_cuda:
+            prompts = not has_kernels(qkv.dtype, self.head_dim)
         out = qk_norm_rope_paged(
             qkv.view(n, -1), self.n_heads, self.n_kv_heads, self.head_dim, self.q_norm.scale, self.k_norm.scale, cos, sin,
-            step.plan.positions, step.plan.slots, layer.k_pages, layer.v_pages, eps=self.q_norm.eps, return_kv=packed,
+            step.plan.positions, step.plan.slots, layer.k_pages, layer.v_pages, eps=self.q_norm.eps, return_kv=prompts,
         )
         window = self.window_size if self.window_size > 0 else -1
-        if packed:
+        if prompts:
             q, k, v = (t.unsqueeze(0) for t in out)
-            out = self.attention(q, k, v, causal=True, window_size=(window, -1), doc_ids=step.doc_ids)
+            if dense:
+                out = self.attention(q, k, v, causal=True, window_size=(window, -1), doc_ids=step.doc_ids)
+            else:
+                out, end = torch.zeros_like(q), 0
+                for length in step.new_lens:
+                    at, end = slice(end, end + length), end + length
+                    if length:
+                        out[:, at] = self.attention(q[:, at], k[:, at], v[:, at], causal=True, window_size=(window, -1))
         else:
             out = paged_attention(out, layer.k_pages, layer.v_pages, step.block_tables, step.plan.positions,
                                   step.plan.rows, window_left=window, alibi_slopes=slopes)

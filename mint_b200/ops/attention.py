@@ -112,10 +112,15 @@ class _FlashAttnFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+def has_kernel(dtype: torch.dtype, head_dim: int) -> bool:
+    """Whether :func:`attention` of CUDA tensors with as many queries as keys runs the FlashAttention kernel
+    (without an explicit mask or bias), or PyTorch code with a materialized mask."""
+    return _ext.kernels_enabled() and dtype == torch.bfloat16 and head_dim == 128
+
+
 def _kernel_supported(q: torch.Tensor, k: torch.Tensor) -> bool:
     return (
-        q.dtype in (torch.bfloat16,)
-        and q.shape[-1] == 128
+        has_kernel(q.dtype, q.shape[-1])
         and k.shape[-1] == 128
         and q.shape[2] % k.shape[2] == 0
         and q.shape[1] == k.shape[1]

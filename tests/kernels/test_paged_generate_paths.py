@@ -1,9 +1,10 @@
-"""generate_batch on the GPU for head sizes without paged kernels, and with the kernels switched off."""
+"""generate_batch on the GPU for head sizes without paged or dense kernels, and with the kernels switched off."""
 
 import pytest
 import torch
 
 from mint_b200.models.gemma import Gemma, GemmaConfig
+from mint_b200.ops import _ext
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +49,15 @@ def test_bf16_heads_without_a_paged_kernel():
     with torch.autocast("cuda", dtype=torch.bfloat16):
         got = model.generate_batch(prompts, 6, temperature=0, max_batch=3)
         _check_tokens(model, prompts, got, 6, 0.05)
+
+
+@pytest.mark.parametrize("head_dim", [64, 256])
+@pytest.mark.parametrize("pattern", ["SL", "L"])
+def test_prompts_of_other_head_sizes_run_kernels(head_dim, pattern):
+    model, prompts = _model(head_dim=head_dim, attention_pattern=pattern), _prompts(1, 200, 33, 7, 129)
+    _ext.reset_fallbacks()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = model.generate_batch(prompts, 10, temperature=0, max_batch=4)
+        assert not _ext.fallback_counts()
+        _check_tokens(model, prompts, got, 10, 0.05)
+    _ext.check_device_status()
