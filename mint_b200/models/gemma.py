@@ -448,9 +448,11 @@ class _Decoder:
 
     def _capture(self) -> None:
         """Capture on a stream of the cache's device: torch's default capture stream is on the device that was
-        current at the process's first capture, and kernels launched on another device would not be recorded."""
+        current at the process's first capture, and kernels launched on another device would not be recorded.
+        Other threads' CUDA calls (a data loader's pinned copies, another model's allocations) do not concern it."""
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=torch.cuda.Stream(self.device)):
+        stream = torch.cuda.Stream(self.device)
+        with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
             self.logits = self._run()
         self.graph = graph
 

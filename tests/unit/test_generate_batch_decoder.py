@@ -86,3 +86,11 @@ def test_only_steps_of_kernels_are_captured(dtype, head_dim, kernels, graph, mon
 
 def _model_stub():
     return type("Stub", (), {"_before_forward": None})()
+
+
+def test_other_threads_calls_do_not_end_the_capture(fake_cuda):
+    decoder = _decoder()
+    with torch.no_grad():
+        for _ in range(2):
+            decoder.step([0, 1], [5, 6])
+    assert fake_cuda["graphs"][0][1]["capture_error_mode"] == "thread_local"
