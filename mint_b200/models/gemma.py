@@ -198,7 +198,8 @@ class Gemma(nn.Module):
         select: torch.Tensor | None = None,
     ) -> torch.Tensor:
         """Logits of every token, or (``select``: token indices) of some. With a paged cache ``input_ids`` is the
-        packed row ``[1, N]`` of a :class:`~mint_b200.kvcache.paged.PagedStep` and ``kv_caches`` its layers."""
+        packed row ``[1, N]`` of a :class:`~mint_b200.kvcache.paged.PagedStep` and ``kv_caches`` its layers; the
+        step has the positions and requests, so ``start_pos``, ``doc_ids`` and ``attn_mask`` are refused."""
         hn = self._trunk(input_ids, kv_caches, start_pos, doc_ids, attn_mask)
         if select is not None:
             hn = hn[:, select]

@@ -145,6 +145,8 @@ class GroupedQueryAttention(nn.Module):
         doc_ids: torch.Tensor | None = None,
     ) -> torch.Tensor:
         if isinstance(kv_cache, PagedLayer):
+            if start_pos != 0 or base_attn_mask is not None or doc_ids is not None:
+                raise ValueError("a paged step has its own positions and requests: no start_pos, attention mask or doc_ids")
             return self._forward_paged(x, kv_cache)
         dt = compute_dtype(x)
         # TP on CUDA: QKV GEMM with its all-gather (SP) or backward all-reduce (no SP), wo GEMM with its

@@ -48,3 +48,13 @@ def test_prompts_attend_one_by_one_without_a_kernel(pattern, monkeypatch):
 def test_what_the_dense_kernel_takes(dtype, head_dim, switch, want, monkeypatch):
     monkeypatch.setenv("MINT_DISABLE_KERNELS", switch)
     assert dense_ops.has_kernel(dtype, head_dim) == want
+
+
+@pytest.mark.parametrize("kw", [{"start_pos": 3}, {"doc_ids": torch.zeros(1, 4, dtype=torch.int32)},
+                                {"attn_mask": torch.ones(1, 1, 4, 4, dtype=torch.bool)}])
+def test_positions_masks_and_documents_next_to_a_step_are_refused(kw):
+    model = Gemma(GemmaConfig(embed_dim=64, hidden_dim=128, seq_length=48, vocab_size=100, n_layers=2, n_heads=4,
+                              n_kv_heads=2, head_dim=16)).eval()
+    step = PagedKVCache(2, 4, 8, 2, 16, max_batch=1, max_seq_len=16).plan([4])
+    with torch.no_grad(), pytest.raises(ValueError, match="positions and requests"):
+        model(torch.zeros(1, 4, dtype=torch.int64), kv_caches=step.layers, **kw)
