@@ -79,10 +79,14 @@ _DOC_CACHE: dict = {}
 
 def _doc_inputs(doc_ids: torch.Tensor | None) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """int32 document ids and their per-token ``[start, end)`` runs, computed once per ids tensor
-    (every layer, forward and backward, shares them). The kernels skip key / query tiles outside
-    each tile's documents when a row's ids are sorted."""
+    (every layer, forward and backward, shares them; every call for inference tensors, which have no
+    version that would show a change). The kernels skip key / query tiles outside each tile's documents
+    when a row's ids are sorted."""
     if doc_ids is None:
         return None, None
+    if doc_ids.is_inference():
+        d = doc_ids.to(torch.int32).contiguous()
+        return d, _ext.require().doc_bounds(d.view(d.shape[0], -1))
     key = (id(doc_ids), doc_ids._version, doc_ids.data_ptr(), tuple(doc_ids.shape))
     hit = _DOC_CACHE.get("entry")
     if hit is not None and hit[0] == key and hit[1]() is doc_ids:
