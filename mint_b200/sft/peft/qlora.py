@@ -10,6 +10,7 @@ dtype and adds the LoRA branch; only ``lora_A`` / ``lora_B`` train.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Any
 
@@ -31,6 +32,13 @@ BLOCK = 64
 SCALE_BLOCK = 256
 
 
+@functools.cache
+def _levels(device: torch.device) -> torch.Tensor:
+    """The levels on ``device``, copied there once: a copy from pageable memory cannot be captured in a CUDA graph."""
+    with torch.inference_mode(False):
+        return NF4_LEVELS.to(device)
+
+
 def nf4_quantize(w: torch.Tensor) -> dict[str, Any]:
     flat = w.detach().float().reshape(-1)
     n = flat.numel()
@@ -40,7 +48,7 @@ def nf4_quantize(w: torch.Tensor) -> dict[str, Any]:
     blocks = flat.view(-1, BLOCK)
     absmax = blocks.abs().amax(dim=1).clamp_min(1e-12)
     normed = blocks / absmax[:, None]
-    levels = NF4_LEVELS.to(w.device)
+    levels = _levels(w.device)
     idx = (normed.unsqueeze(-1) - levels).abs().argmin(dim=-1).to(torch.uint8).reshape(-1)
     packed = (idx[0::2] << 4) | idx[1::2]
     # double quantization of the absmax scales
@@ -58,7 +66,7 @@ def nf4_quantize(w: torch.Tensor) -> dict[str, Any]:
 def nf4_dequantize(q: dict[str, Any], dtype: torch.dtype = torch.float32) -> torch.Tensor:
     packed = q["packed"]
     idx = torch.stack([packed >> 4, packed & 0xF], dim=1).reshape(-1).long()
-    levels = NF4_LEVELS.to(packed.device)
+    levels = _levels(packed.device)
     scales = (q["scale_q"].float().view(-1, SCALE_BLOCK) / 127 * q["scale_max"][:, None]).reshape(-1)
     absmax = scales[: q["nblocks"]] + q["scale_offset"]
     vals = levels[idx].view(-1, BLOCK) * absmax[:, None]

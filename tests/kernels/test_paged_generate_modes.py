@@ -1,10 +1,12 @@
-"""generate_batch on the GPU under inference mode."""
+"""generate_batch on the GPU under inference mode and with adapters."""
 
 import pytest
 import torch
 
 from mint_b200.models.gemma import Gemma, GemmaConfig
 from mint_b200.ops import _ext
+from mint_b200.sft.peft.lora import LoRA
+from mint_b200.sft.peft.qlora import QLoRA
 
 pytestmark = pytest.mark.gpu
 
@@ -27,4 +29,16 @@ def test_inference_mode_changes_nothing():
             got = model.generate_batch(PROMPTS, 12, temperature=0)
         again = model.generate_batch(PROMPTS, 12, temperature=0)
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
+    _ext.check_device_status()
+
+
+@pytest.mark.parametrize("adapter", [LoRA, QLoRA])
+def test_models_with_adapters(adapter):
+    model = _model()
+    adapter.apply(model)
+    model.cuda().eval()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = model.generate_batch(PROMPTS, 12, temperature=0)
+        want = model.generate_batch(PROMPTS, 12, temperature=0, cuda_graph=False)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
     _ext.check_device_status()
