@@ -852,6 +852,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& kp, const at::
                            const at::Tensor& positions, const c10::optional<at::Tensor>& rows, int64_t window,
                            const c10::optional<at::Tensor>& slopes, double scale) {
   paged::check_inference("paged_attention", {&q, &kp, &vp});
+  if (slopes.has_value()) paged::check_inference("paged_attention", {&*slopes});
   check_contig(q, "q");
   check_cuda(tables, "block_tables");
   check_contig(positions, "positions");

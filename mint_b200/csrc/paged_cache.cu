@@ -436,6 +436,8 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
                                            const at::Tensor& slots, at::Tensor& kp, at::Tensor& vp, double eps,
                                            bool dense) {
   paged::check_inference("qk_norm_rope_paged", {&qkv, &qs, &ks, &kp, &vp});
+  if (cos_t.has_value()) paged::check_inference("qk_norm_rope_paged", {&*cos_t});
+  if (sin_t.has_value()) paged::check_inference("qk_norm_rope_paged", {&*sin_t});
   check_cuda(qkv, "qkv");
   check_contig(positions, "positions");
   check_contig(slots, "slots");

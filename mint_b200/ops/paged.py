@@ -175,7 +175,7 @@ def qk_norm_rope_paged(
                                                     k_pages, v_pages, eps, return_kv)
             return tuple(out) if return_kv else out[0]
         _ext.fallback("qk_norm_rope_paged", "dtype / head_dim without a kernel")
-    _inference_only("qk_norm_rope_paged", qkv, q_scale, k_scale, k_pages, v_pages)
+    _inference_only("qk_norm_rope_paged", qkv, q_scale, k_scale, cos, sin, k_pages, v_pages)
     if qkv.dim() != 2 or qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
         raise ValueError(f"qkv must be [N, {(n_q + 2 * n_kv) * head_dim}], got {tuple(qkv.shape)}")
     if k_pages.dtype != qkv.dtype or v_pages.dtype != qkv.dtype:
