@@ -167,6 +167,8 @@ def qk_norm_rope_paged(
     rotation. Norm and rotation are computed in fp32 and rounded once. A token with slot -1 is not
     stored; one whose position or slot is out of range is not stored either and is reported in the
     device status word (CPU tensors raise ValueError)."""
+    if (cos is None) != (sin is None):
+        raise ValueError("qk_norm_rope_paged: rotation needs both cos and sin")
     if _ext.use_cuda_kernels(qkv):
         if qkv.dtype in _KERNEL_DTYPES and head_dim in _HEAD_DIMS:
             if q_scale.dtype != torch.float32 or k_scale.dtype != torch.float32:

@@ -1,0 +1,25 @@
+"""Operands of the paged operators that are easy to get half right."""
+
+import pytest
+import torch
+
+from mint_b200.ops import qk_norm_rope_paged
+
+
+def _append(dev, dtype, **over):
+    i32 = {"dtype": torch.int32, "device": dev}
+    f = {"dtype": dtype, "device": dev}
+    args = {"qkv": torch.randn(1, 3 * 64, **f), "n_q": 1, "n_kv": 1, "head_dim": 64,
+            "q_scale": torch.zeros(64, device=dev), "k_scale": torch.zeros(64, device=dev),
+            "cos": torch.ones(4, 32, device=dev), "sin": torch.zeros(4, 32, device=dev),
+            "positions": torch.arange(1, **i32), "slots": torch.arange(1, **i32),
+            "k_pages": torch.randn(3, 1, 8, 64, **f), "v_pages": torch.randn(3, 1, 8, 64, **f)}
+    return qk_norm_rope_paged(**{**args, **over})
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("missing", ["cos", "sin"])
+def test_half_a_rotation_is_refused(dev, missing):
+    """cos without sin, or sin without cos, which was taken for no rotation."""
+    with pytest.raises(ValueError, match="both cos and sin"):
+        _append(dev, torch.bfloat16, **{missing: None})
