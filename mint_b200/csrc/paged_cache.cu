@@ -448,7 +448,7 @@ std::vector<at::Tensor> qk_norm_rope_paged(const at::Tensor& qkv, int64_t n_q, i
              "qk_norm_rope_paged takes bf16 or fp16 heads of 64, 128 or 256");
   MINT_CHECK(n_q >= 1 && n_kv >= 1 && qkv.dim() == 2 && qkv.size(1) == (n_q + 2 * n_kv) * D, "qkv must be [N, ",
              (n_q + 2 * n_kv) * D, "]");
-  MINT_CHECK(qkv.stride(1) == 1 && qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+  MINT_CHECK(qkv.stride(1) == 1 && (qkv.size(0) <= 1 || qkv.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
              "qkv rows must be contiguous and 16-byte aligned");
   const int64_t N = qkv.size(0);
   MINT_CHECK(positions.scalar_type() == at::kInt && slots.scalar_type() == at::kInt && positions.numel() == N &&

@@ -23,3 +23,11 @@ def test_half_a_rotation_is_refused(dev, missing):
     """cos without sin, or sin without cos, which was taken for no rotation."""
     with pytest.raises(ValueError, match="both cos and sin"):
         _append(dev, torch.bfloat16, **{missing: None})
+
+
+@pytest.mark.gpu
+def test_one_token_may_have_any_row_stride():
+    wide = torch.randn(1, 3 * 64 + 3, device="cuda", dtype=torch.bfloat16)
+    row = wide[:, : 3 * 64]
+    assert row.stride(0) % 8
+    assert torch.equal(_append("cuda", torch.bfloat16, qkv=row), _append("cuda", torch.bfloat16, qkv=row.contiguous()))
