@@ -194,9 +194,11 @@ def _attention_ref(q, k_pages, v_pages, block_tables, positions, rows, window_le
     pos = torch.where((rows >= 0) & (rows < block_tables.shape[0]), positions.long(), -1)
     out = torch.zeros_like(q)
     for i in range(n):  # one query at a time: memory stays at one request's keys
-        last = min(int(pos[i]), block_tables.shape[1] * page_size - 1)
+        last = int(pos[i])
         if last < 0:
             continue
+        if last >= block_tables.shape[1] * page_size:
+            raise ValueError(f"paged_attention: position {last} is beyond block_tables ({block_tables.shape[1]} pages)")
         first = max(0, last - window_left) if window_left >= 0 else 0
         j = torch.arange(first, last + 1, device=q.device)
         page = block_tables[rows[i], j // page_size].long()
@@ -230,7 +232,10 @@ def paged_attention(
     ``window_left >= 0``); each KV head serves ``Hq / Hkv`` query heads. ``alibi_slopes`` (fp32 [Hq])
     adds ``slope * (j - position)`` to the scores. Queries with position -1 (or a row out of range)
     return zeros. Whatever the pages hold outside the keys seen is ignored, NaN included. Several
-    queries of one request may be passed: each is computed on its own."""
+    queries of one request may be passed: each is computed on its own.
+
+    A position beyond the table, or a page beyond the pool among the keys seen, raises ValueError for CPU
+    tensors; on CUDA it is "bad kernel argument" in the device status word, and that output means nothing."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if _ext.use_cuda_kernels(q):
         if q.dtype in _KERNEL_DTYPES and q.shape[-1] in _HEAD_DIMS:

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mint_b200.ops import qk_norm_rope_paged
+from mint_b200.ops import paged_attention, qk_norm_rope_paged
 
 
 def _append(dev, dtype, **over):
@@ -31,3 +31,14 @@ def test_one_token_may_have_any_row_stride():
     row = wide[:, : 3 * 64]
     assert row.stride(0) % 8
     assert torch.equal(_append("cuda", torch.bfloat16, qkv=row), _append("cuda", torch.bfloat16, qkv=row.contiguous()))
+
+
+def test_positions_beyond_the_table_are_refused():
+    """They were answered with the keys that the table does have."""
+    i32 = {"dtype": torch.int32}
+    pool = torch.randn(3, 2, 8, 16)
+    q = torch.randn(2, 4, 16)
+    table = torch.tensor([[0, 1], [2, 0]], **i32)
+    assert paged_attention(q, pool, pool, table, torch.tensor([15, -1], **i32))[0].any()
+    with pytest.raises(ValueError, match="beyond block_tables"):
+        paged_attention(q, pool, pool, table, torch.tensor([16, 3], **i32))
