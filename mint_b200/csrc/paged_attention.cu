@@ -29,7 +29,7 @@
 //   nothing: columns 4-7 of the N block repeat the rows, carry lo where columns 0-3 carry hi, and are added when
 //   the item ends. Scores, sums and outputs are fp32.
 //
-// Measured: 64 requests of 1024 to 32768 keys (16 heads over 4 of 128, pages of 16, 2.2 GB) 331 us, 6.7 TB/s, the
+// Measured in CUDA graphs: 64 requests of 1024 to 32768 keys (16 heads over 4 of 128, pages of 16, 2.2 GB) 331 us, 6.7 TB/s, the
 // rate of a plain copy; the same with 8-line pages 90 % of it. Short work is bound by the chain of dependent reads
 // (position, table entry, keys: 0.65 us each), the merge and the join: one tile takes 5.2 us, a ragged batch of
 // 44 MB in windows of 512 15.6 us, one request of 131072 keys 51 us (41 us at the copy rate). Two CTAs per SM with

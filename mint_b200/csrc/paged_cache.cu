@@ -60,7 +60,8 @@ struct PlanParams {
 // the tokens, tables and request rows, so no block waits for another: a token that falls into a page
 // handed out in this step reads the page id from the free list, not from the table entry that another
 // block writes. A few KB to a few MB move: the bound is the launch and two dependent reads from L2 (lengths,
-// then table or free list). 32 requests with a token each: 3.4 us; 256 prompts of 131 thousand tokens: 5.8 us.
+// then table or free list). In a CUDA graph 32 requests with a
+// token each take 3.4 us, 256 prompts of 131 thousand tokens 5.8 us.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p) {
   extern __shared__ int s_prefix[];  // [B + 1] tokens before request b, [B + 1] fresh pages before it
   int* s_tok = s_prefix;
@@ -298,8 +299,9 @@ __device__ __forceinline__ void write_row(const AppendParams& p, const Place& t,
 
 // A group of lanes takes ROWS consecutive rows (heads) of one token: all their loads are issued before the
 // first reduction, and position, slot, cosines and sines are read once for them. The floor is one read and one
-// write of every row; 65536 tokens of 16 + 8 heads of 128 take 149 us (5.4 TB/s, 82 % of a plain copy; copying
-// the rows to the same places without the arithmetic takes 121 us). What is left is waiting: cosines are read
+// write of every row; 65536 tokens of 16 + 8 heads of 128 take 149 us in a CUDA graph (5.4 TB/s, 82 % of a plain copy;
+// copying the rows to the same places without the arithmetic takes 121 us) and 152 to 164 us as eager calls; with k and
+// v returned as well 166 us (86 %). What is left is waiting: cosines are read
 // after the position, with 28 warps per SM to hide it. Measured and dropped: four rows per group (163 us, fewer
 // warps), persistent warps fed by bulk copies into shared memory (150 us, and far slower for narrow tokens).
 // Few tokens are bound by those two dependent reads: 1 token 2.4 us, 64 tokens 2.4 us.
