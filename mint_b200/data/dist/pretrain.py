@@ -16,6 +16,7 @@ pinned batches, copied to the device every step like real data.
 
 from __future__ import annotations
 
+import atexit
 import queue
 import random
 import threading
@@ -28,6 +29,20 @@ import torch
 from mint_b200.data.dataloader import DataloaderConfig, DistributedDataloader
 from mint_b200.data.packing import BestFitBuffer, pack_row
 from mint_b200.utils.logger import logger
+
+
+_PREFETCHING: dict[threading.Thread, threading.Event] = {}  # running producer threads and what stops them
+
+
+@atexit.register
+def _stop_prefetching() -> None:
+    """End the producer threads before the interpreter does: a daemon thread that it ends inside a torch call
+    takes the process down with "terminate called without an active exception"."""
+    running = list(_PREFETCHING.items())
+    for _thread, stop in running:
+        stop.set()
+    for thread, _stop in running:
+        thread.join(timeout=5.0)  # one that waits for shards may not come back
 
 
 def prefetch(source: Iterator, depth: int) -> Generator:
@@ -53,8 +68,11 @@ def prefetch(source: Iterator, depth: int) -> Generator:
             put(done)
         except BaseException as exc:  # noqa: BLE001
             put(exc)
+        finally:
+            _PREFETCHING.pop(threading.current_thread(), None)
 
     thread = threading.Thread(target=worker, daemon=True)
+    _PREFETCHING[thread] = stop
     thread.start()
     try:
         while True:
