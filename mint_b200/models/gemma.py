@@ -14,6 +14,7 @@ LM head are vocab-parallel and ``forward`` all-gathers the vocabulary shards.
 
 from __future__ import annotations
 
+import functools
 from collections.abc import Sequence
 from dataclasses import dataclass, field
 from typing import Any
@@ -426,6 +427,11 @@ def _sample(logits: torch.Tensor, temperature: float, top_k: int | None, top_p: 
     return torch.multinomial(torch.softmax(logits, dim=-1), num_samples=1)
 
 
+@functools.cache
+def _capture_stream(device: torch.device) -> torch.cuda.Stream:
+    return torch.cuda.Stream(device)
+
+
 class _Decoder:
     """Single-token steps of the running requests of a paged cache, padded to ``max_batch`` tokens. On one
     CUDA GPU, with a cache that the paged kernels take (bf16 / fp16, heads of 64, 128 or 256), the second step is
@@ -451,8 +457,7 @@ class _Decoder:
         """Capture on a stream of the cache's device: torch's default capture stream is on the device that was
         current at the process's first capture, and kernels launched on another device would not be recorded.
         Other threads' CUDA calls (a data loader's pinned copies, another model's allocations) do not concern it."""
-        graph = torch.cuda.CUDAGraph()
-        stream = torch.cuda.Stream(self.device)
+        graph, stream = torch.cuda.CUDAGraph(), _capture_stream(self.device)
         with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
             self.logits = self._run()
         self.graph = graph
